@@ -38,6 +38,7 @@ typedef int ncm_status;
 #define NCM_TYPE_Q8_0 8
 #define NCM_TYPE_Q4_K 12
 #define NCM_TYPE_Q6_K 14
+#define NCM_TYPE_BF16 30
 
 const char* ncm_last_error(void);
 int ncm_version(void);
@@ -109,6 +110,80 @@ ncm_status ncm_attention_kv(int kind, float* out, const float* q, const void* k_
  * score it reads.  The launch is stream ordered and does not synchronise. */
 ncm_status ncm_attention_noalloc(float* out, const float* q, const float* k_cache, const float* v_cache, int pos,
                                  int heads, int kv_heads, int head_dim, void* stream);
+
+/* ---------------------------------------------------------------- batched serving
+ * No counterpart in the reference, whose cache is one contiguous range per session.
+ * A paged cache holds the keys and values of many sequences in pages of page_size tokens;
+ * a sequence's page table lists its pages in order (page_table[sequence][table_width]).
+ * The calls below are stream ordered, allocate nothing and do not synchronise, so they can
+ * be captured into a CUDA graph; lengths, page tables and cu_* arrays are read on the
+ * device.  All pointers must be device memory of the current device (checked: NCM_EINVAL),
+ * and `stream` one of its streams.  16-bit values are rounded to nearest.
+ *
+ * What only the device can see is reported in *err (device int, zeroed by the caller; may
+ * be NULL), whose bits are or-ed: NCM_DEVICE_BAD_ARG for a position, length, cu_* entry or
+ * page id out of its range (no such access is made), NCM_DEVICE_TIMEOUT for a copy that
+ * never arrived (the outputs are then undefined). */
+#define NCM_DEVICE_TIMEOUT 1
+#define NCM_DEVICE_BAD_ARG 4
+
+typedef struct {
+    int32_t type;       /* NCM_TYPE_F16, NCM_TYPE_BF16 or NCM_TYPE_Q8_0 */
+    int32_t page_size;  /* tokens per page: a power of two from 8 to 256 */
+    int32_t kv_heads;
+    int32_t head_dim;   /* 64 or 128 */
+    int64_t pages;
+    int64_t page_stride; /* elements from one page to the next in k and in v, a multiple of 16;
+                            0: kv_heads * page_size * head_dim.  Lets K and V share pages. */
+    void* k;            /* [pages][kv_heads][page_size][head_dim] 16-bit values, or int8 for Q8_0 */
+    void* v;
+    void* k_scales;     /* Q8_0: f16 [pages][kv_heads][page_size][head_dim / 32], else NULL */
+    void* v_scales;
+} ncm_paged_kv;
+
+/* Writes `tokens` new rows into the cache and rotates q on the way.  Row i belongs to the
+ * sequence s with cu_tokens[s] <= i < cu_tokens[s+1] (cu_tokens NULL: sequence i, one row
+ * each); rows outside are padding and left alone.  lengths[s] counts the cached tokens
+ * including the new ones, so that the last new row has position lengths[s] - 1.
+ *   q_out[i] = R(q[i]);  cache K[pos] = R(k[i]);  cache V[pos] = v[i]
+ * in f32 (unfused multiplies and adds), rounded once.  q, k, v are of in_type (F32, F16 or
+ * BF16), rows of heads x head_dim, consecutive rows *_stride elements apart (0: dense), so
+ * slices of one projection's output can be passed; 16-byte aligned.  q_out is a dense
+ * [tokens][heads][head_dim] of q_out_type (F16 or BF16); heads 0 appends without a q.  q_out
+ * may be q when types and strides are equal.  No two rows may share a position of a page.
+ * rope: f32 [rope_len][rope_half][2] of (sin, cos) per position, NULL for no rotation.
+ * NCM_ROPE_PAIRS rotates (2i, 2i+1) for i < rope_half (inference.rs:904-933), the rest passes
+ * unchanged; NCM_ROPE_HALVES rotates (i, i + head_dim/2), rope_half = head_dim/2.
+ * Q8_0: as ncm_model_set_kv_cache's store: scale = max|x| / 127 kept as f16 rounded toward
+ * zero, int8 = round-half-away(x * (1 / scale)).  A row whose position or page is out of
+ * range is not written at all (NCM_DEVICE_BAD_ARG). */
+#define NCM_ROPE_PAIRS 0
+#define NCM_ROPE_HALVES 1
+ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, const void* q, int64_t q_stride, const void* k,
+                            int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int q_out_type, int tokens,
+                            int heads, int batch, const int* cu_tokens, const int* lengths, const int* page_table,
+                            int table_width, const float* rope, int rope_len, int rope_half, int rope_style, int* err,
+                            void* stream);
+
+/* Attention of one new token per sequence over a paged cache:
+ *   out[s][h] = sum_j softmax_j(scale * q[s][h] . K_j) V_j over j < lengths[s],
+ * query head h reading key-value head h / (heads / kv_heads).  A sequence of length 0 gets a
+ * row of zeros; rows of the cache behind the length count for nothing, whatever they hold.
+ * q and out are of q_type (F16 or BF16: the cache's type, either one over Q8_0), rows
+ * q_stride / out_stride elements apart (0: dense), 16-byte aligned; out may not overlap q.
+ * Several rows of one sequence (a speculative batch) are passed as sequences of their own
+ * that share a page table row's contents.  table_width * page_size <= 2^22; a longer length
+ * is cut there and a page id out of range reads as zeros (both NCM_DEVICE_BAD_ARG).
+ * scale 0 means 1 / sqrt(head_dim).  Softmax and sums are f32; the result does not depend on
+ * the order in which the parts of a long sequence finish.
+ * workspace: at least ncm_paged_attention_workspace bytes, zeroed once before its first use
+ * (each call leaves its counters zero again); calls that can overlap on the GPU need one
+ * each, calls in stream order, graph replays among them, can share one. */
+ncm_status ncm_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t* bytes);
+ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_stride, const void* q, int64_t q_stride,
+                               int q_type, int batch, int heads, const int* lengths, const int* page_table,
+                               int table_width, float scale, void* workspace, size_t workspace_bytes, int* err,
+                               void* stream);
 
 /* ---------------------------------------------------------------- fixtures
  * Random-init model spec (the five BASELINE configs are random-init shapes). */

@@ -17,7 +17,9 @@ from dataclasses import dataclass, field
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libncm.so")
 
-Q4_0, Q8_0, Q4_K, Q6_K, F32, F16 = 2, 8, 12, 14, 0, 1
+Q4_0, Q8_0, Q4_K, Q6_K, F32, F16, BF16 = 2, 8, 12, 14, 0, 1, 30
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+DEVICE_TIMEOUT, DEVICE_BAD_ARG = 1, 4   # bits of the device error word of the batched serving calls
 REDUCE_FUSED_P2P, REDUCE_NCCL, REDUCE_HOST_CALLBACK = 0, 1, 2
 STEP_QKV, STEP_W13, STEP_WO, STEP_W2 = 0, 1, 2, 3
 PHASE_ATTENTION, PHASE_FFN, PHASE_HEAD = 0, 1, 2   # tp.rs:203-206 ReducePhase, + the head merge
@@ -32,6 +34,19 @@ class NcmError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"{STATUS.get(status, status)}: {msg}")
         self.status = status
+
+
+class PagedKV(ctypes.Structure):
+    """ncm_paged_kv: a paged key-value cache of type F16, BF16 or Q8_0 (device pointers)."""
+    _fields_ = [("type", ctypes.c_int32), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("pages", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p)]
+
+    def __init__(self, type, k_ptr, v_ptr, pages, page_size, kv_heads, head_dim, k_scales_ptr=0, v_scales_ptr=0,
+                 page_stride=0):
+        super().__init__(type, page_size, kv_heads, head_dim, pages, page_stride, k_ptr, v_ptr, k_scales_ptr or None,
+                         v_scales_ptr or None)
 
 
 class SynthSpec(ctypes.Structure):
@@ -99,6 +114,11 @@ def lib():
         "ncm_fused_silu_mul": (c_int, [c_p, c_p, c_p, c_int, c_p]),
         "ncm_attention": (c_int, [c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_int, c_p]),
         "ncm_attention_kv": (c_int, [c_int, c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_int, c_p]),
+        "ncm_paged_append": (c_int, [ctypes.POINTER(PagedKV), c_int, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_int,
+                                     c_int, c_int, c_int, c_p, c_p, c_p, c_int, c_p, c_int, c_int, c_int, c_p, c_p]),
+        "ncm_paged_attention_workspace": (c_int, [c_int, c_int, c_int, ctypes.POINTER(ctypes.c_size_t)]),
+        "ncm_paged_attention": (c_int, [ctypes.POINTER(PagedKV), c_p, c_i64, c_p, c_i64, c_int, c_int, c_int, c_p, c_p,
+                                        c_int, c_f, c_p, ctypes.c_size_t, c_p, c_p]),
         "ncm_model_set_kv_cache": (c_int, [c_p, c_int]),
         "ncm_gguf_write_synthetic": (c_int, [ctypes.c_char_p, ctypes.POINTER(SynthSpec), c_int]),
         "ncm_synth_tensor_host": (c_int, [ctypes.POINTER(SynthSpec), ctypes.c_char_p, c_int, c_i64, c_i64, c_i64,
@@ -195,6 +215,31 @@ def attention_kv(kind, out_ptr, q_ptr, k_cache_ptr, v_cache_ptr, pos, heads, kv_
     """inference.rs:4319-4458: attention over an F16 (KV_F16) or Q8_0 (KV_Q8_0) cache."""
     _ck(lib().ncm_attention_kv(kind, out_ptr, q_ptr, k_cache_ptr, v_cache_ptr, pos, heads, kv_heads, head_dim,
                                _stream(stream)))
+
+
+# ---------------------------------------------------------------- batched serving (device pointers)
+def paged_append(kv, in_type, q_ptr, k_ptr, v_ptr, q_out_ptr, q_out_type, tokens, heads, batch, cu_tokens_ptr,
+                 lengths_ptr, page_table_ptr, table_width, rope_ptr=0, rope_len=0, rope_half=0, rope_style=ROPE_PAIRS,
+                 q_stride=0, k_stride=0, v_stride=0, err_ptr=0, stream=0):
+    """Rotates the new rows' q and k and stores k and v in a PagedKV cache (include/ncm.h)."""
+    _ck(lib().ncm_paged_append(kv, in_type, q_ptr, q_stride, k_ptr, k_stride, v_ptr, v_stride, q_out_ptr, q_out_type,
+                               tokens, heads, batch, cu_tokens_ptr or None, lengths_ptr, page_table_ptr, table_width,
+                               rope_ptr or None, rope_len, rope_half, rope_style, err_ptr or None, stream or None))
+
+
+def paged_attention_workspace(heads, kv_heads, head_dim):
+    """Bytes of the workspace of paged_attention, which is zeroed before its first use."""
+    n = ctypes.c_size_t()
+    _ck(lib().ncm_paged_attention_workspace(heads, kv_heads, head_dim, ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention(out_ptr, q_ptr, kv, q_type, batch, heads, lengths_ptr, page_table_ptr, table_width, workspace_ptr,
+                    workspace_bytes, scale=0.0, q_stride=0, out_stride=0, err_ptr=0, stream=0):
+    """Attention of one new token per sequence over a PagedKV cache (include/ncm.h)."""
+    _ck(lib().ncm_paged_attention(kv, out_ptr, out_stride, q_ptr, q_stride, q_type, batch, heads, lengths_ptr,
+                                  page_table_ptr, table_width, scale, workspace_ptr, workspace_bytes, err_ptr or None,
+                                  stream or None))
 
 
 # ---------------------------------------------------------------- host helpers

@@ -25,6 +25,7 @@ static ncm_status fail(ncm_status code, const std::string& msg) {
     g_err = msg;
     return code;
 }
+int ncm::set_error(int code, const char* msg) { return fail(code, msg); }
 #define CK(x)                                                                                   \
     do {                                                                                        \
         cudaError_t e_ = (x);                                                                   \

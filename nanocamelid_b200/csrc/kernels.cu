@@ -48,7 +48,7 @@ int num_sms() {
 
 // Raises a kernel's dynamic shared-memory limit once per (kernel, device): the attribute
 // is per device, and several host threads (one per shard) may launch at once.
-static int set_smem_limit(const void* fn, int bytes) {
+int set_smem_limit(const void* fn, int bytes) {
     static std::mutex mu;
     static std::set<std::pair<const void*, int>> done;
     int dev = 0;

@@ -255,6 +255,12 @@ int block_sums_launch(const int8_t* xq, int64_t nblocks, int* xsum, cudaStream_t
 int embed_rows_launch(int type, const uint8_t* table, int64_t pitch, int emb, const int* toks, int ntok,
                       float* hidden, cudaStream_t s, bool pdl);
 int num_sms();
+// Raises a kernel's dynamic shared-memory limit once per (kernel, device).
+int set_smem_limit(const void* fn, int bytes);
+// Sets ncm_last_error() of the calling thread and returns `code` (engine.cu).
+int set_error(int code, const char* msg);
+// Whether p is device memory of the current device (0), else a message (paged.cu).
+const char* device_pointer_error(const void* p);
 // The glibc expf exception table: at most kExpfTabEntries {key, value} pairs, kept in a
 // fixed in-library device array.
 constexpr uint32_t kExpfTabEntries = 1u << 20;
