@@ -154,8 +154,8 @@ typedef struct {
  * rope: f32 [rope_len][rope_half][2] of (sin, cos) per position, NULL for no rotation.
  * NCM_ROPE_PAIRS rotates (2i, 2i+1) for i < rope_half (inference.rs:904-933), the rest passes
  * unchanged; NCM_ROPE_HALVES rotates (i, i + head_dim/2), rope_half = head_dim/2.
- * Q8_0: as ncm_model_set_kv_cache's store: scale = max|x| / 127 kept as f16 rounded toward
- * zero, int8 = round-half-away(x * (1 / scale)).  A row whose position or page is out of
+ * Q8_0: per 32 values scale = max|x| * (1 / 127) in f32, kept as f16 rounded toward zero, int8 =
+ * round-half-away(x * (1 / scale)): ncm_model_set_kv_cache's rule but for its division.  A row whose position or page is out of
  * range is not written at all (NCM_DEVICE_BAD_ARG). */
 #define NCM_ROPE_PAIRS 0
 #define NCM_ROPE_HALVES 1

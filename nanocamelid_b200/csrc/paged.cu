@@ -106,8 +106,10 @@ __device__ __forceinline__ void store8(bool bf16, void* p, const float* x) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack2(bf16, x[0], x[1]), pack2(bf16, x[2], x[3]),
                                               pack2(bf16, x[4], x[5]), pack2(bf16, x[6], x[7]));
 }
-// One 8-value part of a Q8_0 block whose four parts lie in four neighbouring lanes
-// (quantize_row_to_q8_0_blocks: see kv_store_kernel).  All lanes of the warp take part.
+// One 8-value part of a Q8_0 block whose four parts lie in four neighbouring lanes.  The scale
+// is the largest magnitude times 1 / 127: a multiply where the contiguous cache's store divides
+// (kv_store_kernel), one f32 step apart at most before both are cut to f16's eleven bits.
+// All lanes of the warp take part.
 __device__ __forceinline__ void store_q8(bool active, int8_t* values, __half* scale, const float* x, int part) {
     float mx = 0.0f;
 #pragma unroll
@@ -115,7 +117,7 @@ __device__ __forceinline__ void store_q8(bool active, int8_t* values, __half* sc
     mx = fmaxf(mx, __shfl_xor_sync(NCM_FULL, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(NCM_FULL, mx, 2));
     if (!active) return;
-    const float sc = mx / 127.0f, inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+    const float sc = mx * (1.0f / 127.0f), inv = sc > 0.0f ? 1.0f / sc : 0.0f;
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

@@ -306,7 +306,7 @@ def rotated32(x, sc, style, half):
 def quantised(y):
     """Q8_0 of f32 rows by the rule of the header: int8 values and f16 scales (bits)."""
     blk = y.reshape(y.shape[:-1] + (-1, 32))
-    sc = (np.abs(blk).max(-1) / np.float32(127)).astype(np.float32)
+    sc = (np.abs(blk).max(-1) * (np.float32(1) / np.float32(127))).astype(np.float32)
     with np.errstate(divide="ignore", over="ignore"):
         inv = np.where(sc > 0, np.float32(1) / sc, np.float32(0)).astype(np.float32)
     t = (blk * inv[..., None]).astype(np.float32).astype(np.float64)
