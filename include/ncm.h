@@ -185,6 +185,24 @@ ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_st
                                int table_width, float scale, void* workspace, size_t workspace_bytes, int* err,
                                void* stream);
 
+/* Attention over whole prompts (inference.rs:3695-4111 prefill_pass_batch runs its rows one by
+ * one): packed sequences, of which sequence s has the queries cu_q[s] <= i < cu_q[s+1] and the
+ * keys cu_k[s] <= j < cu_k[s+1] (batch + 1 entries each, from 0, not falling; cu_k may be cu_q):
+ *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j
+ * over the sequence's keys; with causal != 0 its last query sees its last key, the one before
+ * one key less, and so on, so that a chunk of a prompt can be passed with all keys before it.
+ * A query that sees no key gets zeros.  Keys that a row does not see do not change it, NaN and
+ * infinities among them.  Rows of out that belong to no sequence are left alone.
+ * q and out: [total_q][heads][head_dim], k and v: [total_k][kv_heads][head_dim], of `type` (F16
+ * or BF16), tokens *_stride elements apart (0: dense), 16-byte aligned; head_dim 64 or 128, at
+ * most 128 query heads to a key-value head; out may not overlap an input.  scale 0 means
+ * 1 / sqrt(head_dim).  cu_* entries that fall or lie past total_q / total_k are cut to the range
+ * (NCM_DEVICE_BAD_ARG).  Runs on tcgen05; p is rounded to `type`, sums are f32. */
+ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k,
+                                int64_t k_stride, const void* v, int64_t v_stride, int type, int total_q, int total_k,
+                                int batch, int heads, int kv_heads, int head_dim, const int* cu_q, const int* cu_k,
+                                int causal, float scale, int* err, void* stream);
+
 /* ---------------------------------------------------------------- fixtures
  * Random-init model spec (the five BASELINE configs are random-init shapes). */
 typedef struct {

@@ -119,6 +119,8 @@ def lib():
         "ncm_paged_attention_workspace": (c_int, [c_int, c_int, c_int, ctypes.POINTER(ctypes.c_size_t)]),
         "ncm_paged_attention": (c_int, [ctypes.POINTER(PagedKV), c_p, c_i64, c_p, c_i64, c_int, c_int, c_int, c_p, c_p,
                                         c_int, c_f, c_p, ctypes.c_size_t, c_p, c_p]),
+        "ncm_prompt_attention": (c_int, [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64] + [c_int] * 7 +
+                                 [c_p, c_p, c_int, c_f, c_p, c_p]),
         "ncm_model_set_kv_cache": (c_int, [c_p, c_int]),
         "ncm_gguf_write_synthetic": (c_int, [ctypes.c_char_p, ctypes.POINTER(SynthSpec), c_int]),
         "ncm_synth_tensor_host": (c_int, [ctypes.POINTER(SynthSpec), ctypes.c_char_p, c_int, c_i64, c_i64, c_i64,
@@ -240,6 +242,15 @@ def paged_attention(out_ptr, q_ptr, kv, q_type, batch, heads, lengths_ptr, page_
     _ck(lib().ncm_paged_attention(kv, out_ptr, out_stride, q_ptr, q_stride, q_type, batch, heads, lengths_ptr,
                                   page_table_ptr, table_width, scale, workspace_ptr, workspace_bytes, err_ptr or None,
                                   stream or None))
+
+
+def prompt_attention(out_ptr, q_ptr, k_ptr, v_ptr, type, total_q, total_k, batch, heads, kv_heads, head_dim, cu_q_ptr,
+                     cu_k_ptr, causal=True, scale=0.0, q_stride=0, k_stride=0, v_stride=0, out_stride=0, err_ptr=0,
+                     stream=0):
+    """Attention over whole packed prompts, causal or not (include/ncm.h)."""
+    _ck(lib().ncm_prompt_attention(out_ptr, out_stride, q_ptr, q_stride, k_ptr, k_stride, v_ptr, v_stride, type, total_q,
+                                   total_k, batch, heads, kv_heads, head_dim, cu_q_ptr, cu_k_ptr, int(causal), scale,
+                                   err_ptr or None, stream or None))
 
 
 # ---------------------------------------------------------------- host helpers

@@ -16,7 +16,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libncm.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CU_SOURCES = ["kernels.cu", "engine.cu", "paged.cu"]
+CU_SOURCES = ["kernels.cu", "engine.cu", "paged.cu", "prompt.cu"]
 CPP_SOURCES = ["gguf.cpp", "libm_table.cpp"]
 
 

@@ -1,0 +1,590 @@
+// Attention over whole prompts: packed sequences of different lengths, grouped heads, causal
+// or not, on the tcgen05 tensor cores.
+//
+//   out_i = sum_j softmax_j(scale * q_i . k_j) v_j
+//
+// One CTA per SM walks over work items.  An item is one key-value head of one sequence and
+// 2 x 128 query rows, a row being one (token, head of the group): all heads of a group share
+// the K and V tiles, and a short prompt still fills the tile's rows.  Twelve warps:
+//   0-3, 4-7  softmax of query tile 0 / 1, one thread per row: scores from TMEM, maximum,
+//             exponentials, p back into TMEM (over the scores), and at the end the output;
+//   8         TMA: queries, then K and V tiles of 128 keys into a ring;
+//   9         one thread issues the tensor-core products S = Q K^T and O += P V;
+//   10, 11    look over the V tiles at the mask's edge: a row that a mask hides has p = 0, but
+//             0 x infinity is not 0, so what is not finite there is taken out and given back
+//             in the epilogue to the rows that do see it.
+// While one tile's softmax runs, the tensor cores work on the other's products.
+// TMEM: columns 0, 128: S (and P) of the two tiles; 256, 384: O.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cuda_fp16.h>
+#include <cuda_bf16.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+#include <algorithm>
+#include "../../include/ncm.h"
+#include "ncm_internal.h"
+#include "common.cuh"
+
+namespace ncm {
+namespace {
+
+constexpr int kRows = 128;               // query rows of a tile, and keys of a tile
+constexpr int kPromptThreads = 384;
+constexpr int kPromptBatch = 2048;       // sequences of one launch
+constexpr int kPromptSmem = 232448;
+constexpr uint64_t kPromptWaitNs = 2000000000ull;
+
+struct alignas(64) PromptParams {
+    CUtensorMap qm;                      // {hd, group, kv_heads, tokens}, box {64, group, 1, tokens of a tile}
+    CUtensorMap km, vm;                  // {hd, kv_heads, tokens}, box {64, 1, 128}
+    void* out;
+    const void* v;
+    int64_t out_stride, v_stride;        // elements between tokens
+    const int *cu_q, *cu_k;
+    int batch, kv_heads, group, tokens;  // tokens: of a tile, 128 / group
+    int total_q, total_k, causal;
+    float scale_log2;
+    int* err;
+};
+
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Shared-memory operand descriptors, 128-byte swizzle, in units of 16 bytes.  Rows of 128 bytes
+// in groups of eight (1024 bytes apart).  K-major (Q, K): the leading offset is not used.
+// MN-major (V: keys x d, d contiguous): 64 values of d lie in one 128-byte row; the next 64 lie
+// `lead` bytes on, the next eight keys 1024 bytes on.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+// Instruction descriptor of kind::f16: f32 accumulators, A and B f16 or bf16, M 128, N, B K-major or MN-major.
+__host__ __device__ constexpr uint32_t inst_desc(bool bf16, int n, bool b_mn) {
+    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (b_mn ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t inst, bool add) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+        ::"r"(d), "l"(a), "l"(b), "r"(inst), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t inst, bool add) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
+        ::"r"(d), "r"(a), "l"(b), "r"(inst), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define NCM_R8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
+#define NCM_W8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+// 32 columns of this warp's 32 lanes (one row per lane).
+__device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : NCM_W8(r, 0), NCM_W8(r, 8), NCM_W8(r, 16), NCM_W8(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::NCM_R8(r, 0), NCM_R8(r, 8), NCM_R8(r, 16), NCM_R8(r, 24), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::NCM_R8(r, 0), NCM_R8(r, 8), "r"(addr) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16> __device__ __forceinline__ float widen(uint16_t h) {
+    return BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+}
+// Whether one of the 16-bit floats in w is infinite or NaN: its exponent's ones carry into bit 15.
+template <bool BF16> __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return BF16 ? ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+
+// What every role knows of an item.
+struct Item {
+    int b, head;              // sequence, key-value head
+    int q0, nq, k0, nk;       // first row and rows of the sequence in q and in k
+    int t0;                   // first token of tile 0 within the sequence
+    int shift;                // causal: token t sees keys up to t + shift
+    int n[2];                 // key tiles of each query tile
+    int clear;                // key tiles below this are not cut by the mask for any row of the item
+};
+__device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix, int index) {
+    Item t;
+    const int block = prefix[p.batch] - 1 - index / p.kv_heads;   // the blocks that see most keys come first
+    t.head = index % p.kv_heads;
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= block) lo = mid; else hi = mid;
+    }
+    t.b = lo;
+    const int2 q = make_int2(__ldg(p.cu_q + lo), __ldg(p.cu_q + lo + 1)), k = make_int2(__ldg(p.cu_k + lo), __ldg(p.cu_k + lo + 1));
+    t.q0 = min(max(q.x, 0), p.total_q); t.nq = min(max(q.y, t.q0), p.total_q) - t.q0;
+    t.k0 = min(max(k.x, 0), p.total_k); t.nk = min(max(k.y, t.k0), p.total_k) - t.k0;
+    t.t0 = (block - prefix[lo]) * 2 * p.tokens;
+    t.shift = t.nk - t.nq;
+    int least = t.nk;                                             // keys that every row sees
+    for (int x = 0; x < 2; ++x) {
+        const int first = t.t0 + x * p.tokens, last = min(first + p.tokens, t.nq) - 1;
+        int end = 0;
+        if (first <= last) {
+            end = p.causal ? min(t.nk, last + t.shift + 1) : t.nk;
+            if (p.causal) least = min(least, first + t.shift + 1);
+        }
+        t.n[x] = end > 0 ? (end + kRows - 1) / kRows : 0;
+    }
+    t.clear = max(least, 0) / kRows;
+    return t;
+}
+// Items are dealt out in rows of one per CTA, every other row backwards: the work of an item
+// falls along the list, and this evens out what the CTAs get.
+__device__ __forceinline__ int item_index(int it) {
+    return it * gridDim.x + ((it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+template <bool BF16, int HD>
+struct Layout {
+    static constexpr int kTile = kRows * HD * 2;            // bytes of a tile of Q, K or V
+    static constexpr int kStages = HD == 128 ? 4 : 8;
+    static constexpr int kRing = 2 * kTile;
+    static constexpr int kBars = kRing + kStages * kTile;   // barriers, then a few words, then prefix
+    static constexpr int kWords = kBars + 8 * (3 * kStages + 8);
+    static constexpr int kPrefix = kWords + 4 * 32;
+};
+
+template <bool BF16, int HD>
+__global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __grid_constant__ PromptParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    using L = Layout<BF16, HD>;
+    constexpr int NST = L::kStages, SLABS = HD / 64, SLAB = kRows * 128;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+    uint64_t *empty = full + NST, *edge = empty + NST, *q_full = edge + NST, *q_empty = q_full + 1, *s_ready = q_empty + 1,
+             *p_ready = s_ready + 2, *o_ready = p_ready + 2;
+    uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::kWords);   // [0] TMEM address, [8..16) items with odd V, [16..) sums
+    int* prefix = reinterpret_cast<int*>(smem + L::kPrefix);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity, kPromptWaitNs)) {
+            ok = false;
+            set_dev_error(p.err, NCM_DEVERR_MBAR_TIMEOUT);
+        }
+        return ok;
+    };
+
+    // ---- barriers, TMEM, and the running sum of blocks of 2 tiles over the sequences
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(words)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < NST; ++i) { mbar_init(full + i, 2); mbar_init(empty + i, 1); mbar_init(edge + i, 1); }
+        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        for (int x = 0; x < 2; ++x) { mbar_init(s_ready + x, 1); mbar_init(p_ready + x, 4); mbar_init(o_ready + x, 1); }
+        fence_mbar_init();
+    }
+    if (tid < 8) words[8 + tid] = 0;
+    {
+        const int per = (p.batch + kPromptThreads - 1) / kPromptThreads, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+        int sum = 0;
+        for (int b = b0; b < b1; ++b) {
+            const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1), k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
+            if (blockIdx.x == 0 && (q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k))
+                set_dev_error(p.err, NCM_DEVERR_BAD_ARG);
+            const int at = min(max(q0, 0), p.total_q), n = min(max(q1, at), p.total_q) - at;
+            prefix[b + 1] = (n + 2 * p.tokens - 1) / (2 * p.tokens);
+            sum += prefix[b + 1];
+        }
+        int run = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(NCM_FULL, run, o);
+            if (lane >= o) run += v;
+        }
+        if (lane == 31) words[16 + warp] = run;
+        __syncthreads();
+        run -= sum;
+        for (int w = 0; w < warp; ++w) run += words[16 + w];
+        if (tid == 0) prefix[0] = 0;
+        for (int b = b0; b < b1; ++b) { run += prefix[b + 1]; prefix[b + 1] = run; }
+        fence_before();
+        __syncthreads();
+        fence_after();
+    }
+    const int items = prefix[p.batch] * p.kv_heads;
+    const uint32_t tmem = words[0];
+    const uint32_t q_smem = smem_u32(smem), ring = q_smem + L::kRing;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8 && lane == 0) {
+            // ---- TMA
+            uint32_t slot = 0, round = 0, quse = 0;
+            // A V tile at the mask's edge goes to warps 10 and 11, which pass it on: `full` takes
+            // their two arrivals, or two from here.
+            auto load = [&](const CUtensorMap* m, const Item& t, int j, bool at_edge) {
+                if (!wait(empty + slot, (round & 1) ^ 1)) return;
+                uint64_t* bar = (at_edge ? edge : full) + slot;
+                if (!at_edge) mbar_arrive(bar);
+                mbar_arrive_expect_tx(bar, L::kTile);
+                for (int s = 0; s < SLABS; ++s) tma3(ring + slot * L::kTile + s * SLAB, m, bar, 64 * s, t.head, t.k0 + j * kRows);
+                if (++slot == NST) { slot = 0; ++round; }
+            };
+            for (int it = 0; ok; ++it) {
+                const int index = item_index(it);
+                if (it * (int)gridDim.x >= items) break;
+                if (index >= items) continue;
+                const Item t = item_at(p, prefix, index);
+                const int n = max(t.n[0], t.n[1]);
+                if (n == 0) continue;
+                if (!wait(q_empty, (quse & 1) ^ 1)) break;
+                ++quse;
+                const int box = p.tokens * p.group * 128;
+                mbar_arrive_expect_tx(q_full, ((t.n[0] > 0) + (t.n[1] > 0)) * SLABS * box);
+                for (int x = 0; x < 2; ++x)
+                    if (t.n[x] > 0)
+                        for (int s = 0; s < SLABS; ++s)
+                            tma4(q_smem + x * L::kTile + s * SLAB, &p.qm, q_full, 64 * s, 0, t.head, t.q0 + t.t0 + x * p.tokens);
+                for (int j = 0; j < n && ok; ++j) { load(&p.km, t, j, false); load(&p.vm, t, j, j >= t.clear); }
+            }
+            // every stage is given back before the CTA ends
+            for (int i = 0; i < NST && ok; ++i) {
+                wait(empty + slot, (round & 1) ^ 1);
+                if (++slot == NST) { slot = 0; ++round; }
+            }
+            wait(q_empty, (quse & 1) ^ 1);
+        } else if (warp == 9 && lane == 0) {
+            // ---- products
+            constexpr uint32_t inst_s = inst_desc(BF16, kRows, false), inst_o = inst_desc(BF16, HD, true);
+            uint32_t base = 0, quse = 0, puse[2] = {0, 0};
+            auto slot_of = [&](uint32_t i) { return (base + i) % NST; };
+            auto phase_of = [&](uint32_t i) { return ((base + i) / NST) & 1; };
+            auto scores = [&](int x, uint32_t i) {
+                const uint32_t a = q_smem + x * L::kTile, b = ring + slot_of(i) * L::kTile;
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint32_t off = (k / 4) * SLAB + (k % 4) * 32;
+                    mma_ss(tmem + x * 128, smem_desc(a + off, 16), smem_desc(b + off, 16), inst_s, k > 0);
+                }
+                mma_commit(s_ready + x);
+            };
+            for (int it = 0; ok; ++it) {
+                const int index = item_index(it);
+                if (it * (int)gridDim.x >= items) break;
+                if (index >= items) continue;
+                const Item t = item_at(p, prefix, index);
+                const int n = max(t.n[0], t.n[1]);
+                if (n == 0) continue;
+                if (!wait(q_full, quse & 1)) break;
+                ++quse;
+                if (!wait(full + slot_of(0), phase_of(0))) break;
+                fence_after();
+                for (int x = 0; x < 2; ++x)
+                    if (t.n[x] > 0) scores(x, 0);
+                mma_commit(empty + slot_of(0));
+                if (n == 1) mma_commit(q_empty);
+                for (int j = 0; j < n && ok; ++j) {
+                    const uint32_t vi = 2 * j + 1, ki = 2 * j + 2;
+                    const uint32_t vs = slot_of(vi);
+                    wait(full + vs, phase_of(vi));
+                    if (j + 1 < n) wait(full + slot_of(ki), phase_of(ki));
+                    for (int x = 0; x < 2 && ok; ++x) {
+                        if (j >= t.n[x]) continue;
+                        if (!wait(p_ready + x, puse[x] & 1)) break;
+                        ++puse[x];
+                        fence_after();
+#pragma unroll
+                        for (int k = 0; k < kRows / 16; ++k)
+                            mma_ts(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, smem_desc(ring + vs * L::kTile + k * 2048, SLAB),
+                                   inst_o, j > 0 || k > 0);
+                        if (j + 1 < t.n[x]) scores(x, ki);
+                        else mma_commit(o_ready + x);
+                    }
+                    mma_commit(empty + vs);
+                    if (j + 1 < n) mma_commit(empty + slot_of(ki));
+                    if (j + 2 == n) mma_commit(q_empty);
+                }
+                base += 2 * n;
+            }
+        } else if (warp >= 10) {
+            // ---- V tiles at the mask's edge
+            uint32_t base = 0, phases = 0;   // bit s: parity of edge[s]'s next phase
+            for (int it = 0; ok; ++it) {
+                const int index = item_index(it);
+                if (it * (int)gridDim.x >= items) break;
+                if (index >= items) continue;
+                const Item t = item_at(p, prefix, index);
+                const int n = max(t.n[0], t.n[1]);
+                for (int j = t.clear; j < n && ok; ++j) {
+                    const uint32_t s = (base + 2 * j + 1) % NST;
+                    if (!wait(edge + s, (phases >> s) & 1)) break;
+                    phases ^= 1u << s;
+                    uint4* tile = reinterpret_cast<uint4*>(smem + L::kRing + s * L::kTile);
+                    uint32_t odd = 0;
+#pragma unroll 8
+                    for (int e = (warp - 10) * 32 + lane; e < L::kTile / 16; e += 64) {
+                        const uint4 w = tile[e];
+                        odd |= not_finite<BF16>(w.x) | not_finite<BF16>(w.y) | not_finite<BF16>(w.z) | not_finite<BF16>(w.w);
+                    }
+                    if (__any_sync(NCM_FULL, odd)) {
+                        for (int e = (warp - 10) * 32 + lane; e < L::kTile / 16; e += 64) {
+                            uint32_t* w = reinterpret_cast<uint32_t*>(tile + e);
+                            for (int c = 0; c < 4; ++c) {
+                                const uint32_t bits = not_finite<BF16>(w[c]);
+                                if (bits & 0x8000u) w[c] &= 0xffff0000u;
+                                if (bits & 0x80000000u) w[c] &= 0x0000ffffu;
+                            }
+                        }
+                        if (lane == 0) words[8 + (it & 7)] = it + 1;
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + s);
+                }
+                base += 2 * n;
+            }
+        }
+    } else {
+        // ---- softmax, one row per thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int x = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // 32 lanes per warp, in bits 16 and up
+        const uint32_t s_at = tmem + x * 128 + lanes, o_at = tmem + 256 + x * 128 + lanes;
+        const int token = row / p.group, member = row % p.group;
+        uint32_t suse = 0, ouse = 0;
+        for (int it = 0; ok; ++it) {
+            const int index = item_index(it);
+            if (it * (int)gridDim.x >= items) break;
+            if (index >= items) continue;
+            const Item t = item_at(p, prefix, index);
+            const int at = t.t0 + x * p.tokens + token;                 // token within the sequence
+            const bool mine = token < p.tokens && at < t.nq;
+            const int limit = !mine ? -1 : p.causal ? min(at + t.shift, t.nk - 1) : t.nk - 1;   // last key seen
+            float top = -INFINITY, sum = 0.0f;                          // running maximum (times scale, log2), sum of p
+            for (int j = 0; j < t.n[x]; ++j) {
+                if (!wait(s_ready + x, suse & 1)) break;
+                ++suse;
+                fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, s_at + 32 * c);
+                wait_ld();
+                if (j >= t.clear) {
+                    const int left = limit - j * kRows;                 // columns up to this one are seen
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c > left) s[c] = 0xff800000u;
+                }
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 128; ++c) m[c & 3] = fmaxf(m[c & 3], __uint_as_float(s[c]));
+                const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * p.scale_log2;
+                // The maximum is moved only where a score has passed it by more than 2^8, so that
+                // the sums in TMEM are rarely rescaled; p stays below 2^8.
+                const bool over = now > top + 8.0f;
+                if (__any_sync(NCM_FULL, over)) {
+                    const float a = over ? ex2(top - now) : 1.0f;
+                    if (over) top = now;
+                    sum *= a;
+                    if (j > 0) {   // the products before these scores are complete, so O is at rest
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o, o_at + c);
+                            wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                            tmem_st32(o_at + c, o);
+                        }
+                    }
+                }
+                const float shift = top == -INFINITY ? 0.0f : -top;
+                float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float a = ex2(fmaf(__uint_as_float(s[32 * c + 2 * i]), p.scale_log2, shift));
+                        const float b = ex2(fmaf(__uint_as_float(s[32 * c + 2 * i + 1]), p.scale_log2, shift));
+                        l[(2 * i) & 3] += a; l[(2 * i + 1) & 3] += b;
+                        w[i] = pack<BF16>(a, b);
+                    }
+                    tmem_st16(s_at + 16 * c, w);
+                }
+                sum += (l[0] + l[1]) + (l[2] + l[3]);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + x);
+            }
+            if (t.n[x] > 0) {
+                if (!wait(o_ready + x, ouse & 1)) break;
+                ++ouse;
+                fence_after();
+            }
+            const bool odd = words[8 + (it & 7)] == (uint32_t)(it + 1);
+            const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;   // a row without keys: zeros
+            uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)(t.q0 + at) * p.out_stride + (int64_t)(t.head * p.group + member) * HD;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                if (t.n[x] > 0) {
+                    tmem_ld32(o, o_at + c);
+                    wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                if (odd && mine) {
+                    // infinities and NaN that were taken out of V, for the rows that see their keys
+                    const uint16_t* v = static_cast<const uint16_t*>(p.v) + (int64_t)t.k0 * p.v_stride + t.head * HD + c;
+                    for (int key = t.clear * kRows; key <= limit; ++key)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const uint16_t h = __ldg(v + key * p.v_stride + i);
+                            if (not_finite<BF16>(h)) o[i] = __float_as_uint(__uint_as_float(o[i]) + widen<BF16>(h));
+                        }
+                }
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = pack<BF16>(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(out + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            fence_before();   // O is read before the next item's products overwrite it
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ------------------------------------------------------------------ host side
+bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
+int bad(const char* what) { return set_error(NCM_EINVAL, what); }
+
+bool kv_map(CUtensorMap* m, const void* base, int hd, int kv_heads, int tokens, int64_t stride) {
+    const cuuint64_t dim[3] = {(cuuint64_t)hd, (cuuint64_t)kv_heads, (cuuint64_t)tokens};
+    const cuuint64_t step[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, kRows}, one[3] = {1, 1, 1};
+    return encode_tiled_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dim, step, box, one,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool q_map(CUtensorMap* m, const void* base, int hd, int group, int kv_heads, int tokens, int64_t stride, int box_tokens) {
+    const cuuint64_t dim[4] = {(cuuint64_t)hd, (cuuint64_t)group, (cuuint64_t)kv_heads, (cuuint64_t)tokens};
+    const cuuint64_t step[3] = {(cuuint64_t)hd * 2, (cuuint64_t)group * hd * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)box_tokens}, one[4] = {1, 1, 1, 1};
+    return encode_tiled_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dim, step, box, one,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int HD>
+int prompt_run(const PromptParams& p, int grid, cudaStream_t s) {
+    const int bytes = Layout<BF16, HD>::kPrefix + 4 * (p.batch + 1);
+    auto fn = prompt_attn_kernel<BF16, HD>;
+    if (int r = set_smem_limit((const void*)fn, kPromptSmem)) return r;
+    fn<<<grid, kPromptThreads, bytes, s>>>(p);
+    return (int)cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace ncm
+
+using namespace ncm;
+
+extern "C" ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k,
+                                           int64_t k_stride, const void* v, int64_t v_stride, int type, int total_q,
+                                           int total_k, int batch, int heads, int kv_heads, int head_dim, const int* cu_q,
+                                           const int* cu_k, int causal, float scale, int* err, void* stream) {
+    if (type != NCM_TYPE_F16 && type != NCM_TYPE_BF16) return bad("type must be F16 or BF16");
+    if (head_dim != 64 && head_dim != 128) return bad("head_dim must be 64 or 128");
+    if (heads < 1 || kv_heads < 1 || kv_heads > 1024 || heads % kv_heads || heads / kv_heads > 128)
+        return bad("heads must be a multiple of kv_heads, 128 to one at most");
+    if (total_q < 0 || total_k < 0 || batch < 0 || total_q > (1 << 30) || total_k > (1 << 30)) return bad("bad prompt sizes");
+    if (!(scale >= 0.0f) || scale > 3.0e38f) return bad("scale must be positive (0: 1 / sqrt(head_dim))");
+    if (total_q == 0 || batch == 0) return NCM_OK;
+    if (!out || !q || !cu_q || !cu_k || (total_k && (!k || !v))) return bad("null pointer");
+    const int64_t wide_q = (int64_t)heads * head_dim, wide_k = (int64_t)kv_heads * head_dim;
+    int64_t* stride[4] = {&out_stride, &q_stride, &k_stride, &v_stride};
+    const void* at[4] = {out, q, k, v};
+    for (int i = 0; i < 4; ++i) {
+        const int64_t wide = i < 2 ? wide_q : wide_k;
+        if (!*stride[i]) *stride[i] = wide;
+        if (*stride[i] < wide || *stride[i] % 8 || *stride[i] > ((int64_t)1 << 38) || !aligned16(at[i]))
+            return bad("rows must be 16-byte aligned and at least a token apart");
+    }
+    if (total_k == 0) { k = q; v = q; k_stride = q_stride; v_stride = q_stride; }   // never read: no row sees a key
+    const void* check[] = {out, q, k, v, cu_q, cu_k};
+    for (const void* c : check)
+        if (const char* e = device_pointer_error(c)) return bad(e);
+    if (!encode_tiled_fn()) return set_error(NCM_ECUDA, "cuTensorMapEncodeTiled not available");
+    PromptParams p;
+    memset(&p, 0, sizeof p);
+    p.group = heads / kv_heads;
+    p.tokens = kRows / p.group;
+    if (!q_map(&p.qm, q, head_dim, p.group, kv_heads, total_q, q_stride, p.tokens) ||
+        !kv_map(&p.km, k, head_dim, kv_heads, std::max(total_k, 1), k_stride) ||
+        !kv_map(&p.vm, v, head_dim, kv_heads, std::max(total_k, 1), v_stride))
+        return set_error(NCM_ECUDA, "cuTensorMapEncodeTiled failed for the prompt");
+    p.out = out; p.v = v; p.out_stride = out_stride; p.v_stride = v_stride;
+    p.kv_heads = kv_heads; p.total_q = total_q; p.total_k = total_k; p.causal = causal != 0;
+    p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
+    p.err = err;
+    cudaStream_t s = (cudaStream_t)stream;
+    for (int b = 0; b < batch; b += kPromptBatch) {
+        p.batch = std::min(kPromptBatch, batch - b);
+        p.cu_q = cu_q + b; p.cu_k = cu_k + b;
+        const int64_t most = ((int64_t)total_q / (2 * p.tokens) + p.batch) * kv_heads;
+        if (most > (1 << 30)) return set_error(NCM_EUNSUPPORTED, "too many blocks of queries");
+        const int grid = (int)std::min<int64_t>(num_sms(), most);
+        int r;
+        if (type == NCM_TYPE_BF16) r = head_dim == 64 ? prompt_run<true, 64>(p, grid, s) : prompt_run<true, 128>(p, grid, s);
+        else r = head_dim == 64 ? prompt_run<false, 64>(p, grid, s) : prompt_run<false, 128>(p, grid, s);
+        if (r) return set_error(NCM_ECUDA, cudaGetErrorString((cudaError_t)r));
+    }
+    return NCM_OK;
+}

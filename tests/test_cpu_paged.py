@@ -69,9 +69,27 @@ def test_attention_refusals(ncm, kw):
     refused(ncm, attend, cache(ncm), **kw)
 
 
+def prompt(ncm, **kw):
+    a = dict(out_ptr=P, q_ptr=P, k_ptr=P, v_ptr=P, type=ncm.F16, total_q=8, total_k=8, batch=2, heads=4, kv_heads=2,
+             head_dim=64, cu_q_ptr=P, cu_k_ptr=P)
+    a.update(kw)
+    ncm.prompt_attention(**a)
+
+
+@pytest.mark.parametrize("kw", [dict(type=0), dict(type=8), dict(head_dim=32), dict(head_dim=256), dict(heads=0), dict(kv_heads=0),
+                                dict(heads=5), dict(heads=258, kv_heads=2), dict(total_q=-1), dict(total_k=-1), dict(batch=-1),
+                                dict(total_q=(1 << 30) + 1), dict(out_ptr=0), dict(q_ptr=0), dict(k_ptr=0), dict(v_ptr=0),
+                                dict(cu_q_ptr=0), dict(cu_k_ptr=0), dict(q_ptr=P + 8), dict(out_ptr=P + 2), dict(k_stride=127),
+                                dict(q_stride=260), dict(out_stride=-256), dict(v_stride=130), dict(scale=-0.5), dict(scale=float("nan"))])
+def test_prompt_refusals(ncm, kw):
+    refused(ncm, prompt, **kw)
+
+
 def test_nothing_to_do_is_no_error(ncm):
     append(ncm, cache(ncm), tokens=0)
     attend(ncm, cache(ncm), batch=0)
+    prompt(ncm, total_q=0)
+    prompt(ncm, batch=0)
 
 
 def test_pointers_that_are_not_device_memory_are_refused(ncm):
