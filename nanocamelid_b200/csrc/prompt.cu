@@ -13,8 +13,8 @@
 //   10, 11    look over the V tiles at the mask's edge: a row that a mask hides has p = 0, but
 //             0 x infinity is not 0, so what is not finite there is taken out and given back
 //             in the epilogue to the rows that do see it.
-// While one tile's softmax runs, the tensor cores work on the other's products.
-// TMEM: columns 0, 128: S (and P) of the two tiles; 256, 384: O.
+// The softmax takes a tile's 128 keys in two steps of 64, whose p the tensor cores take one by
+// one.  TMEM columns: 128 x: S of tile x, and over it P, 64 h the step's; 256 + 128 x: O.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
@@ -30,9 +30,14 @@
 namespace ncm {
 namespace {
 
-constexpr int kRows = 128;               // query rows of a tile, and keys of a tile
+constexpr int kRows = 128;               // query rows of a tile, and keys of a K or V tile
+constexpr int kUnitKeys = 64;            // keys of one step of the softmax
 constexpr int kPromptThreads = 384;
 constexpr int kPromptBatch = 2048;       // sequences of one launch
+#ifndef POLY8
+#define POLY8 2
+#endif
+constexpr int kPolyOf8 = POLY8;
 constexpr int kPromptSmem = 232448;
 constexpr uint64_t kPromptWaitNs = 2000000000ull;
 
@@ -58,6 +63,13 @@ __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* m, uint64_
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
         ::"r"(dst), "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// One lane of a converged warp, in a form that the compiler knows for one: the operands of the
+// instructions under it stay in uniform registers.
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(yes));
+    return yes != 0;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -118,6 +130,57 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two f32 in one 64-bit register, for the packed f32 instructions.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void apart(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two values at or below a few hundred, on the FMA pipe: x = n + f with f in [-1/2, 1/2]
+// by adding and taking off 1.5 * 2^23, a minimax polynomial of 2^f (Remez exchange; relative
+// error 7.5e-5 of degree 3, 2.6e-6 of degree 4, against roundings of 2^-9 and 2^-12 that
+// follow), n added to the exponent.  Below 2^-126 it gives 2^-126.
+template <bool BF16> __device__ __forceinline__ void ex2_poly(uint64_t x2, float& lo, float& hi) {
+    float a, b;
+    apart(x2, a, b);
+    x2 = two(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t t = add2(x2, two(12582912.0f, 12582912.0f));
+    const uint64_t f = fma2(add2(t, two(-12582912.0f, -12582912.0f)), two(-1.0f, -1.0f), x2);
+    uint64_t y;
+    if (BF16) {
+        y = two(0x1.c3f760p-5f, 0x1.c3f760p-5f);
+        y = fma2(y, f, two(0x1.f0de1ap-3f, 0x1.f0de1ap-3f));
+        y = fma2(y, f, two(0x1.62f31ap-1f, 0x1.62f31ap-1f));
+        y = fma2(y, f, two(0x1.fff692p-1f, 0x1.fff692p-1f));
+    } else {
+        y = two(0x1.3997d6p-7f, 0x1.3997d6p-7f);
+        y = fma2(y, f, two(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+        y = fma2(y, f, two(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+        y = fma2(y, f, two(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+        y = fma2(y, f, two(0x1.fffffep-1f, 0x1.fffffep-1f));
+    }
+    float n0, n1;
+    apart(t, n0, n1);
+    apart(y, lo, hi);
+    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(n0) << 23));
+    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n1) << 23));
+}
 template <bool BF16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     if (BF16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -140,8 +203,10 @@ struct Item {
     int q0, nq, k0, nk;       // first row and rows of the sequence in q and in k
     int t0;                   // first token of tile 0 within the sequence
     int shift;                // causal: token t sees keys up to t + shift
-    int n[2];                 // key tiles of each query tile
-    int clear;                // key tiles below this are not cut by the mask for any row of the item
+    int n0, n1;               // units of 64 keys of each query tile
+    __device__ __forceinline__ int n(int x) const { return x ? n1 : n0; }
+    __device__ __forceinline__ int tiles() const { return (max(n0, n1) + 1) / 2; }
+    int seen;                 // keys that every row sees: what lies below is not cut by the mask
 };
 __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix, int index) {
     Item t;
@@ -159,6 +224,7 @@ __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix
     t.t0 = (block - prefix[lo]) * 2 * p.tokens;
     t.shift = t.nk - t.nq;
     int least = t.nk;                                             // keys that every row sees
+#pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int first = t.t0 + x * p.tokens, last = min(first + p.tokens, t.nq) - 1;
         int end = 0;
@@ -166,9 +232,9 @@ __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix
             end = p.causal ? min(t.nk, last + t.shift + 1) : t.nk;
             if (p.causal) least = min(least, first + t.shift + 1);
         }
-        t.n[x] = end > 0 ? (end + kRows - 1) / kRows : 0;
+        (x ? t.n1 : t.n0) = end > 0 ? (end + kUnitKeys - 1) / kUnitKeys : 0;
     }
-    t.clear = max(least, 0) / kRows;
+    t.seen = max(least, 0);
     return t;
 }
 // Items are dealt out in rows of one per CTA, every other row backwards: the work of an item
@@ -183,7 +249,7 @@ struct Layout {
     static constexpr int kStages = HD == 128 ? 4 : 8;
     static constexpr int kRing = 2 * kTile;
     static constexpr int kBars = kRing + kStages * kTile;   // barriers, then a few words, then prefix
-    static constexpr int kWords = kBars + 8 * (3 * kStages + 8);
+    static constexpr int kWords = kBars + 8 * (3 * kStages + 10);
     static constexpr int kPrefix = kWords + 4 * 32;
 };
 
@@ -194,16 +260,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     constexpr int NST = L::kStages, SLABS = HD / 64, SLAB = kRows * 128;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
     uint64_t *empty = full + NST, *edge = empty + NST, *q_full = edge + NST, *q_empty = q_full + 1, *s_ready = q_empty + 1,
-             *p_ready = s_ready + 2, *o_ready = p_ready + 2;
+             *p_ready = s_ready + 2, *pv_done = p_ready + 4;   // [x], [2 x + h], [x]
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::kWords);   // [0] TMEM address, [8..16) items with odd V, [16..) sums
     int* prefix = reinterpret_cast<int*>(smem + L::kPrefix);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(NCM_FULL, tid >> 5, 0), lane = tid & 31;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok && !mbar_wait(bar, parity, kPromptWaitNs)) {
             ok = false;
             set_dev_error(p.err, NCM_DEVERR_MBAR_TIMEOUT);
         }
+        return ok;
+    };
+    // The same for a whole warp, which goes on together: the TMEM instructions want all lanes.
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+        ok = __all_sync(NCM_FULL, wait(bar, parity));
         return ok;
     };
 
@@ -215,7 +286,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) { mbar_init(full + i, 2); mbar_init(empty + i, 1); mbar_init(edge + i, 1); }
         mbar_init(q_full, 1); mbar_init(q_empty, 1);
-        for (int x = 0; x < 2; ++x) { mbar_init(s_ready + x, 1); mbar_init(p_ready + x, 4); mbar_init(o_ready + x, 1); }
+        for (int i = 0; i < 4; ++i) mbar_init(p_ready + i, 4);
+        for (int x = 0; x < 2; ++x) { mbar_init(s_ready + x, 1); mbar_init(pv_done + x, 1); }
         fence_mbar_init();
     }
     if (tid < 8) words[8 + tid] = 0;
@@ -251,7 +323,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + L::kRing;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8 && lane == 0) {
             // ---- TMA
             uint32_t slot = 0, round = 0, quse = 0;
@@ -270,17 +342,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (it * (int)gridDim.x >= items) break;
                 if (index >= items) continue;
                 const Item t = item_at(p, prefix, index);
-                const int n = max(t.n[0], t.n[1]);
+                const int n = t.tiles();
                 if (n == 0) continue;
                 if (!wait(q_empty, (quse & 1) ^ 1)) break;
                 ++quse;
                 const int box = p.tokens * p.group * 128;
-                mbar_arrive_expect_tx(q_full, ((t.n[0] > 0) + (t.n[1] > 0)) * SLABS * box);
+                mbar_arrive_expect_tx(q_full, ((t.n0 > 0) + (t.n1 > 0)) * SLABS * box);
                 for (int x = 0; x < 2; ++x)
-                    if (t.n[x] > 0)
+                    if (t.n(x) > 0)
                         for (int s = 0; s < SLABS; ++s)
                             tma4(q_smem + x * L::kTile + s * SLAB, &p.qm, q_full, 64 * s, 0, t.head, t.q0 + t.t0 + x * p.tokens);
-                for (int j = 0; j < n && ok; ++j) { load(&p.km, t, j, false); load(&p.vm, t, j, j >= t.clear); }
+                for (int j = 0; j < n && ok; ++j) { load(&p.km, t, j, false); load(&p.vm, t, j, j >= t.seen / kRows); }
             }
             // every stage is given back before the CTA ends
             for (int i = 0; i < NST && ok; ++i) {
@@ -288,56 +360,72 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (++slot == NST) { slot = 0; ++round; }
             }
             wait(q_empty, (quse & 1) ^ 1);
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 9) {
             // ---- products
             constexpr uint32_t inst_s = inst_desc(BF16, kRows, false), inst_o = inst_desc(BF16, HD, true);
-            uint32_t base = 0, quse = 0, puse[2] = {0, 0};
+            uint32_t base = 0, quse = 0, phases = 0;   // bit 2 x + h: parity of p_ready's next phase
             auto slot_of = [&](uint32_t i) { return (base + i) % NST; };
             auto phase_of = [&](uint32_t i) { return ((base + i) / NST) & 1; };
             auto scores = [&](int x, uint32_t i) {
                 const uint32_t a = q_smem + x * L::kTile, b = ring + slot_of(i) * L::kTile;
+                if (elected()) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint32_t off = (k / 4) * SLAB + (k % 4) * 32;
-                    mma_ss(tmem + x * 128, smem_desc(a + off, 16), smem_desc(b + off, 16), inst_s, k > 0);
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint32_t off = (k / 4) * SLAB + (k % 4) * 32;
+                        mma_ss(tmem + x * 128, smem_desc(a + off, 16), smem_desc(b + off, 16), inst_s, k > 0);
+                    }
+                    mma_commit(s_ready + x);
                 }
-                mma_commit(s_ready + x);
+                __syncwarp();
             };
             for (int it = 0; ok; ++it) {
                 const int index = item_index(it);
                 if (it * (int)gridDim.x >= items) break;
                 if (index >= items) continue;
                 const Item t = item_at(p, prefix, index);
-                const int n = max(t.n[0], t.n[1]);
+                const int n = t.tiles();
                 if (n == 0) continue;
-                if (!wait(q_full, quse & 1)) break;
+                if (!wait_all(q_full, quse & 1)) break;
                 ++quse;
-                if (!wait(full + slot_of(0), phase_of(0))) break;
+                if (!wait_all(full + slot_of(0), phase_of(0))) break;
                 fence_after();
+#pragma unroll
                 for (int x = 0; x < 2; ++x)
-                    if (t.n[x] > 0) scores(x, 0);
-                mma_commit(empty + slot_of(0));
-                if (n == 1) mma_commit(q_empty);
+                    if (t.n(x) > 0) scores(x, 0);
+                if (elected()) {
+                    mma_commit(empty + slot_of(0));
+                    if (n == 1) mma_commit(q_empty);
+                }
+                __syncwarp();
                 for (int j = 0; j < n && ok; ++j) {
                     const uint32_t vi = 2 * j + 1, ki = 2 * j + 2;
                     const uint32_t vs = slot_of(vi);
-                    wait(full + vs, phase_of(vi));
-                    if (j + 1 < n) wait(full + slot_of(ki), phase_of(ki));
-                    for (int x = 0; x < 2 && ok; ++x) {
-                        if (j >= t.n[x]) continue;
-                        if (!wait(p_ready + x, puse[x] & 1)) break;
-                        ++puse[x];
-                        fence_after();
+                    wait_all(full + vs, phase_of(vi));
+                    if (j + 1 < n) wait_all(full + slot_of(ki), phase_of(ki));
 #pragma unroll
-                        for (int k = 0; k < kRows / 16; ++k)
-                            mma_ts(tmem + 256 + x * 128, tmem + x * 128 + 8 * k, smem_desc(ring + vs * L::kTile + k * 2048, SLAB),
-                                   inst_o, j > 0 || k > 0);
-                        if (j + 1 < t.n[x]) scores(x, ki);
-                        else mma_commit(o_ready + x);
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int u = 2 * j + h;
+                            if (u >= t.n(x) || !wait_all(p_ready + 2 * x + h, (phases >> (2 * x + h)) & 1)) continue;
+                            phases ^= 1u << (2 * x + h);
+                            fence_after();
+                            if (elected()) {
+#pragma unroll
+                                for (int k = 0; k < kUnitKeys / 16; ++k)
+                                    mma_ts(tmem + 256 + x * 128, tmem + x * 128 + h * 64 + 8 * k,
+                                           smem_desc(ring + vs * L::kTile + (4 * h + k) * 2048, SLAB), inst_o, u > 0 || k > 0);
+                                mma_commit(pv_done + x);
+                            }
+                            __syncwarp();
+                            if (h == 1 && u + 1 < t.n(x)) scores(x, ki);
+                        }
+                    if (elected()) {
+                        mma_commit(empty + vs);
+                        if (j + 1 < n) mma_commit(empty + slot_of(ki));
+                        if (j + 2 == n) mma_commit(q_empty);
                     }
-                    mma_commit(empty + vs);
-                    if (j + 1 < n) mma_commit(empty + slot_of(ki));
-                    if (j + 2 == n) mma_commit(q_empty);
+                    __syncwarp();
                 }
                 base += 2 * n;
             }
@@ -349,10 +437,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (it * (int)gridDim.x >= items) break;
                 if (index >= items) continue;
                 const Item t = item_at(p, prefix, index);
-                const int n = max(t.n[0], t.n[1]);
-                for (int j = t.clear; j < n && ok; ++j) {
+                const int n = t.tiles();
+                for (int j = t.seen / kRows; j < n && ok; ++j) {
                     const uint32_t s = (base + 2 * j + 1) % NST;
-                    if (!wait(edge + s, (phases >> s) & 1)) break;
+                    if (!wait_all(edge + s, (phases >> s) & 1)) break;
                     phases ^= 1u << s;
                     uint4* tile = reinterpret_cast<uint4*>(smem + L::kRing + s * L::kTile);
                     uint32_t odd = 0;
@@ -382,12 +470,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
         }
     } else {
         // ---- softmax, one row per thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int x = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // 32 lanes per warp, in bits 16 and up
         const uint32_t s_at = tmem + x * 128 + lanes, o_at = tmem + 256 + x * 128 + lanes;
         const int token = row / p.group, member = row % p.group;
-        uint32_t suse = 0, ouse = 0;
+        uint32_t phases = 0, handed = 0;   // of s_ready; units given to the products
         for (int it = 0; ok; ++it) {
             const int index = item_index(it);
             if (it * (int)gridDim.x >= items) break;
@@ -396,33 +484,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
             const int at = t.t0 + x * p.tokens + token;                 // token within the sequence
             const bool mine = token < p.tokens && at < t.nq;
             const int limit = !mine ? -1 : p.causal ? min(at + t.shift, t.nk - 1) : t.nk - 1;   // last key seen
+            const int units = t.n(x);
             float top = -INFINITY, sum = 0.0f;                          // running maximum (times scale, log2), sum of p
-            for (int j = 0; j < t.n[x]; ++j) {
-                if (!wait(s_ready + x, suse & 1)) break;
-                ++suse;
-                fence_after();
-                uint32_t s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s + 32 * c, s_at + 32 * c);
+            for (int u = 0; u < units; ++u) {
+                const int h = u & 1;
+                const uint32_t s_unit = s_at + 64 * h;
+                if (h == 0) {
+                    if (!wait_all(s_ready + x, phases & 1)) break;
+                    ++phases;
+                    fence_after();
+                }
+                uint32_t s[64];
+                tmem_ld32(s, s_unit);
+                tmem_ld32(s + 32, s_unit + 32);
                 wait_ld();
-                if (j >= t.clear) {
-                    const int left = limit - j * kRows;                 // columns up to this one are seen
+                const bool masked = (u + 1) * kUnitKeys > t.seen;
+                if (masked) {
+                    const int left = limit - u * kUnitKeys;             // columns up to this one are seen
 #pragma unroll
-                    for (int c = 0; c < 128; ++c)
+                    for (int c = 0; c < 64; ++c)
                         if (c > left) s[c] = 0xff800000u;
                 }
-                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float m[4];
 #pragma unroll
-                for (int c = 0; c < 128; ++c) m[c & 3] = fmaxf(m[c & 3], __uint_as_float(s[c]));
-                const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * p.scale_log2;
+                for (int c = 0; c < 4; ++c) m[c] = max3(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]), -INFINITY);
+#pragma unroll
+                for (int c = 8; c < 64; c += 2) m[(c >> 1) & 3] = max3(m[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                const float now = max3(max3(m[0], m[1], m[2]), m[3], -INFINITY) * p.scale_log2;
                 // The maximum is moved only where a score has passed it by more than 2^8, so that
-                // the sums in TMEM are rarely rescaled; p stays below 2^8.
-                const bool over = now > top + 8.0f;
+                // the sums in TMEM are rarely rescaled; p stays below 2^8.  A score that is NaN or
+                // infinite makes the row NaN.
+                const bool over = !(now <= top + 8.0f);
                 if (__any_sync(NCM_FULL, over)) {
-                    const float a = over ? ex2(top - now) : 1.0f;
-                    if (over) top = now;
+                    const float a = !over ? 1.0f : now < INFINITY ? ex2(top - now) : NAN;
+                    if (over && now < INFINITY) top = now;
                     sum *= a;
-                    if (j > 0) {   // the products before these scores are complete, so O is at rest
+                    if (!(now < INFINITY)) sum = NAN;
+                    if (u > 0) {   // O is at rest once the last unit's products are complete (those before it are: S of this unit is here)
+                        if (!wait_all(pv_done + x, (handed - 1) & 1)) break;
+                        fence_after();
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             uint32_t o[32];
@@ -435,28 +535,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                     }
                 }
                 const float shift = top == -INFINITY ? 0.0f : -top;
-                float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                const uint64_t scale2 = two(p.scale_log2, p.scale_log2), shift2 = two(shift, shift);
+                uint64_t l0 = 0, l1 = 0;
+                // p of 32 columns; with a mask by ex2 alone, which gives 0 where it hides
+                auto part = [&](int c, bool plain) {
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float a = ex2(fmaf(__uint_as_float(s[32 * c + 2 * i]), p.scale_log2, shift));
-                        const float b = ex2(fmaf(__uint_as_float(s[32 * c + 2 * i + 1]), p.scale_log2, shift));
-                        l[(2 * i) & 3] += a; l[(2 * i + 1) & 3] += b;
+                        const uint64_t v = fma2(two(__uint_as_float(s[32 * c + 2 * i]), __uint_as_float(s[32 * c + 2 * i + 1])), scale2, shift2);
+                        float a, b;
+                        if (!plain && (i & 7) < kPolyOf8) {
+                            ex2_poly<BF16>(v, a, b);
+                        } else {
+                            apart(v, a, b);
+                            a = ex2(a); b = ex2(b);
+                        }
+                        (i & 1 ? l1 : l0) = add2(i & 1 ? l1 : l0, two(a, b));
                         w[i] = pack<BF16>(a, b);
                     }
-                    tmem_st16(s_at + 16 * c, w);
-                }
-                sum += (l[0] + l[1]) + (l[2] + l[3]);
+                    tmem_st16(s_unit + 16 * c, w);
+                };
+                if (masked) { part(0, true); part(1, true); } else { part(0, false); part(1, false); }
                 wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + x);
+                if (lane == 0) mbar_arrive(p_ready + 2 * x + h);
+                ++handed;
+                float la, lb, lc, ld;
+                apart(l0, la, lb);
+                apart(l1, lc, ld);
+                sum += (la + lb) + (lc + ld);
             }
-            if (t.n[x] > 0) {
-                if (!wait(o_ready + x, ouse & 1)) break;
-                ++ouse;
+            if (units > 0) {   // the last two units' products may both be on the way: one phase after the other
+                if (units > 1 && !wait_all(pv_done + x, handed & 1)) break;
+                if (!wait_all(pv_done + x, (handed - 1) & 1)) break;
                 fence_after();
             }
             const bool odd = words[8 + (it & 7)] == (uint32_t)(it + 1);
@@ -465,7 +577,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
-                if (t.n[x] > 0) {
+                if (units > 0) {
                     tmem_ld32(o, o_at + c);
                     wait_ld();
                 } else {
@@ -475,7 +587,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (odd && mine) {
                     // infinities and NaN that were taken out of V, for the rows that see their keys
                     const uint16_t* v = static_cast<const uint16_t*>(p.v) + (int64_t)t.k0 * p.v_stride + t.head * HD + c;
-                    for (int key = t.clear * kRows; key <= limit; ++key)
+                    for (int key = t.seen / kRows * kRows; key <= limit; ++key)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const uint16_t h = __ldg(v + key * p.v_stride + i);
