@@ -9,11 +9,14 @@
 //   0-3, 4-7  softmax of query tile 0 / 1, one thread per row: scores from TMEM, maximum,
 //             exponentials, p back into TMEM (over the scores), and at the end the output;
 //   8         TMA: queries, then K and V tiles of 128 keys into a ring;
-//   9         one thread issues the tensor-core products S = Q K^T and O += P V;
-//   10, 11    look over the V tiles at the mask's edge: a row that a mask hides has p = 0, but
+//   9         issues the tensor-core products S = Q K^T and O += P V;
+//   10, 11    look over the V tiles at the mask's edge: a key that a mask hides has p = 0, but
 //             0 x infinity is not 0, so what is not finite there is taken out and given back
 //             in the epilogue to the rows that do see it.
-// The softmax takes a tile's 128 keys in two steps of 64, whose p the tensor cores take one by
+// While one tile's softmax runs, the tensor cores work on the other's products.  (A warp of its
+// own for each tile's products was slower, 579 us against 523 at one prompt of 8192, 32 / 8
+// heads of 128; scores in units of 64 keys, double buffered, too: 560 us, since a product
+// with N = 64 takes as long as one with N = 128.)  The softmax takes a tile's 128 keys in two steps of 64, whose p the tensor cores take one by
 // one.  TMEM columns: 128 x: S of tile x, and over it P, 64 h the step's; 256 + 128 x: O.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -33,7 +36,7 @@ namespace {
 constexpr int kRows = 128;               // query rows of a tile, and keys of a K or V tile
 constexpr int kUnitKeys = 64;            // keys of one step of the softmax
 constexpr int kPromptThreads = 384;
-constexpr int kPromptBatch = 2048;       // sequences of one launch
+constexpr int kPromptBatch = 1024;       // sequences of one launch
 #ifndef POLY8
 #define POLY8 2
 #endif
@@ -209,6 +212,7 @@ struct Item {
     int seen;                 // keys that every row sees: what lies below is not cut by the mask
 };
 __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix, int index) {
+    const int *cu_q = prefix + p.batch + 1, *cu_k = cu_q + p.batch + 1;
     Item t;
     const int block = prefix[p.batch] - 1 - index / p.kv_heads;   // the blocks that see most keys come first
     t.head = index % p.kv_heads;
@@ -218,7 +222,7 @@ __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix
         if (prefix[mid] <= block) lo = mid; else hi = mid;
     }
     t.b = lo;
-    const int2 q = make_int2(__ldg(p.cu_q + lo), __ldg(p.cu_q + lo + 1)), k = make_int2(__ldg(p.cu_k + lo), __ldg(p.cu_k + lo + 1));
+    const int2 q = make_int2(cu_q[lo], cu_q[lo + 1]), k = make_int2(cu_k[lo], cu_k[lo + 1]);
     t.q0 = min(max(q.x, 0), p.total_q); t.nq = min(max(q.y, t.q0), p.total_q) - t.q0;
     t.k0 = min(max(k.x, 0), p.total_k); t.nk = min(max(k.y, t.k0), p.total_k) - t.k0;
     t.t0 = (block - prefix[lo]) * 2 * p.tokens;
@@ -235,6 +239,10 @@ __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix
         (x ? t.n1 : t.n0) = end > 0 ? (end + kUnitKeys - 1) / kUnitKeys : 0;
     }
     t.seen = max(least, 0);
+    // the same in all lanes: said in a form that the compiler knows, for uniform registers
+    t.n0 = __shfl_sync(NCM_FULL, t.n0, 0);
+    t.n1 = __shfl_sync(NCM_FULL, t.n1, 0);
+    t.seen = __shfl_sync(NCM_FULL, t.seen, 0);
     return t;
 }
 // Items are dealt out in rows of one per CTA, every other row backwards: the work of an item
@@ -249,8 +257,9 @@ struct Layout {
     static constexpr int kStages = HD == 128 ? 4 : 8;
     static constexpr int kRing = 2 * kTile;
     static constexpr int kBars = kRing + kStages * kTile;   // barriers, then a few words, then prefix
-    static constexpr int kWords = kBars + 8 * (3 * kStages + 10);
-    static constexpr int kPrefix = kWords + 4 * 32;
+    static constexpr int kWords = kBars + 8 * (3 * kStages + 12);
+    static constexpr int kStore = (kWords + 4 * 32 + 127) / 128 * 128;   // 2 KB per softmax warp: 32 rows of 32 output values
+    static constexpr int kPrefix = kStore + 8 * 2048;       // running sums of blocks, cu_q, cu_k: batch + 1 each
 };
 
 template <bool BF16, int HD>
@@ -260,7 +269,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     constexpr int NST = L::kStages, SLABS = HD / 64, SLAB = kRows * 128;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
     uint64_t *empty = full + NST, *edge = empty + NST, *q_full = edge + NST, *q_empty = q_full + 1, *s_ready = q_empty + 1,
-             *p_ready = s_ready + 2, *pv_done = p_ready + 4;   // [x], [2 x + h], [x]
+             *p_ready = s_ready + 2, *pv_done = p_ready + 4, *o_ready = pv_done + 2;   // [x], [2 x + h], [x], [x]
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::kWords);   // [0] TMEM address, [8..16) items with odd V, [16..) sums
     int* prefix = reinterpret_cast<int*>(smem + L::kPrefix);
     const int tid = threadIdx.x, warp = __shfl_sync(NCM_FULL, tid >> 5, 0), lane = tid & 31;
@@ -287,7 +296,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
         for (int i = 0; i < NST; ++i) { mbar_init(full + i, 2); mbar_init(empty + i, 1); mbar_init(edge + i, 1); }
         mbar_init(q_full, 1); mbar_init(q_empty, 1);
         for (int i = 0; i < 4; ++i) mbar_init(p_ready + i, 4);
-        for (int x = 0; x < 2; ++x) { mbar_init(s_ready + x, 1); mbar_init(pv_done + x, 1); }
+        for (int x = 0; x < 2; ++x) { mbar_init(s_ready + x, 1); mbar_init(pv_done + x, 1); mbar_init(o_ready + x, 1); }
         fence_mbar_init();
     }
     if (tid < 8) words[8 + tid] = 0;
@@ -301,6 +310,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
             const int at = min(max(q0, 0), p.total_q), n = min(max(q1, at), p.total_q) - at;
             prefix[b + 1] = (n + 2 * p.tokens - 1) / (2 * p.tokens);
             sum += prefix[b + 1];
+        }
+        for (int b = tid; b <= p.batch; b += kPromptThreads) {
+            prefix[p.batch + 1 + b] = __ldg(p.cu_q + b);
+            prefix[2 * (p.batch + 1) + b] = __ldg(p.cu_k + b);
         }
         int run = sum;
 #pragma unroll
@@ -318,23 +331,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
         __syncthreads();
         fence_after();
     }
-    const int items = prefix[p.batch] * p.kv_heads;
-    const uint32_t tmem = words[0];
+    const int items = __shfl_sync(NCM_FULL, prefix[p.batch] * p.kv_heads, 0);
+    const uint32_t tmem = __shfl_sync(NCM_FULL, words[0], 0);
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + L::kRing;
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
             // ---- TMA
             uint32_t slot = 0, round = 0, quse = 0;
             // A V tile at the mask's edge goes to warps 10 and 11, which pass it on: `full` takes
             // their two arrivals, or two from here.
             auto load = [&](const CUtensorMap* m, const Item& t, int j, bool at_edge) {
-                if (!wait(empty + slot, (round & 1) ^ 1)) return;
+                if (!wait_all(empty + slot, (round & 1) ^ 1)) return;
                 uint64_t* bar = (at_edge ? edge : full) + slot;
-                if (!at_edge) mbar_arrive(bar);
-                mbar_arrive_expect_tx(bar, L::kTile);
-                for (int s = 0; s < SLABS; ++s) tma3(ring + slot * L::kTile + s * SLAB, m, bar, 64 * s, t.head, t.k0 + j * kRows);
+                if (elected()) {
+                    if (!at_edge) mbar_arrive(bar);
+                    mbar_arrive_expect_tx(bar, L::kTile);
+                    for (int s = 0; s < SLABS; ++s) tma3(ring + slot * L::kTile + s * SLAB, m, bar, 64 * s, t.head, t.k0 + j * kRows);
+                }
+                __syncwarp();
                 if (++slot == NST) { slot = 0; ++round; }
             };
             for (int it = 0; ok; ++it) {
@@ -344,28 +360,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 const Item t = item_at(p, prefix, index);
                 const int n = t.tiles();
                 if (n == 0) continue;
-                if (!wait(q_empty, (quse & 1) ^ 1)) break;
+                if (!wait_all(q_empty, (quse & 1) ^ 1)) break;
                 ++quse;
                 const int box = p.tokens * p.group * 128;
-                mbar_arrive_expect_tx(q_full, ((t.n0 > 0) + (t.n1 > 0)) * SLABS * box);
-                for (int x = 0; x < 2; ++x)
-                    if (t.n(x) > 0)
-                        for (int s = 0; s < SLABS; ++s)
-                            tma4(q_smem + x * L::kTile + s * SLAB, &p.qm, q_full, 64 * s, 0, t.head, t.q0 + t.t0 + x * p.tokens);
+                if (elected()) {
+                    mbar_arrive_expect_tx(q_full, ((t.n0 > 0) + (t.n1 > 0)) * SLABS * box);
+                    for (int x = 0; x < 2; ++x)
+                        if (t.n(x) > 0)
+                            for (int s = 0; s < SLABS; ++s)
+                                tma4(q_smem + x * L::kTile + s * SLAB, &p.qm, q_full, 64 * s, 0, t.head, t.q0 + t.t0 + x * p.tokens);
+                }
+                __syncwarp();
                 for (int j = 0; j < n && ok; ++j) { load(&p.km, t, j, false); load(&p.vm, t, j, j >= t.seen / kRows); }
             }
             // every stage is given back before the CTA ends
             for (int i = 0; i < NST && ok; ++i) {
-                wait(empty + slot, (round & 1) ^ 1);
+                wait_all(empty + slot, (round & 1) ^ 1);
                 if (++slot == NST) { slot = 0; ++round; }
             }
-            wait(q_empty, (quse & 1) ^ 1);
+            wait_all(q_empty, (quse & 1) ^ 1);
         } else if (warp == 9) {
             // ---- products
             constexpr uint32_t inst_s = inst_desc(BF16, kRows, false), inst_o = inst_desc(BF16, HD, true);
             uint32_t base = 0, quse = 0, phases = 0;   // bit 2 x + h: parity of p_ready's next phase
-            auto slot_of = [&](uint32_t i) { return (base + i) % NST; };
-            auto phase_of = [&](uint32_t i) { return ((base + i) / NST) & 1; };
+            auto slot_of = [&](uint32_t i) { return (base + i) % NST; };   // K and V tile j: places 2 j and 2 j + 1
+            auto arrived = [&](uint32_t i) { return wait_all(full + slot_of(i), ((base + i) / NST) & 1); };
             auto scores = [&](int x, uint32_t i) {
                 const uint32_t a = q_smem + x * L::kTile, b = ring + slot_of(i) * L::kTile;
                 if (elected()) {
@@ -378,6 +397,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 }
                 __syncwarp();
             };
+            auto give_back = [&](uint64_t* bar) {
+                if (elected()) mma_commit(bar);
+                __syncwarp();
+            };
             for (int it = 0; ok; ++it) {
                 const int index = item_index(it);
                 if (it * (int)gridDim.x >= items) break;
@@ -387,21 +410,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (n == 0) continue;
                 if (!wait_all(q_full, quse & 1)) break;
                 ++quse;
-                if (!wait_all(full + slot_of(0), phase_of(0))) break;
+                if (!arrived(0)) break;
                 fence_after();
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    if (t.n(x) > 0) scores(x, 0);
-                if (elected()) {
-                    mma_commit(empty + slot_of(0));
-                    if (n == 1) mma_commit(q_empty);
-                }
-                __syncwarp();
+                if (t.n0 > 0) scores(0, 0);
+                if (t.n1 > 0) scores(1, 0);
+                give_back(empty + slot_of(0));
+                if (n == 1) give_back(q_empty);
                 for (int j = 0; j < n && ok; ++j) {
-                    const uint32_t vi = 2 * j + 1, ki = 2 * j + 2;
-                    const uint32_t vs = slot_of(vi);
-                    wait_all(full + vs, phase_of(vi));
-                    if (j + 1 < n) wait_all(full + slot_of(ki), phase_of(ki));
+                    if (!arrived(2 * j + 1)) break;
+                    if (j + 1 < n && !arrived(2 * j + 2)) break;
+                    const uint32_t v = ring + slot_of(2 * j + 1) * L::kTile;
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -413,16 +431,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                             if (elected()) {
 #pragma unroll
                                 for (int k = 0; k < kUnitKeys / 16; ++k)
-                                    mma_ts(tmem + 256 + x * 128, tmem + x * 128 + h * 64 + 8 * k,
-                                           smem_desc(ring + vs * L::kTile + (4 * h + k) * 2048, SLAB), inst_o, u > 0 || k > 0);
+                                    mma_ts(tmem + 256 + x * 128, tmem + x * 128 + h * 64 + 8 * k, smem_desc(v + (4 * h + k) * 2048, SLAB), inst_o,
+                                           u > 0 || k > 0);
                                 mma_commit(pv_done + x);
+                                if (u + 1 == t.n(x)) mma_commit(o_ready + x);
                             }
                             __syncwarp();
-                            if (h == 1 && u + 1 < t.n(x)) scores(x, ki);
+                            if (h == 1 && u + 1 < t.n(x)) scores(x, 2 * j + 2);
                         }
                     if (elected()) {
-                        mma_commit(empty + vs);
-                        if (j + 1 < n) mma_commit(empty + slot_of(ki));
+                        mma_commit(empty + slot_of(2 * j + 1));
+                        if (j + 1 < n) mma_commit(empty + slot_of(2 * j + 2));
                         if (j + 2 == n) mma_commit(q_empty);
                     }
                     __syncwarp();
@@ -442,15 +461,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                     const uint32_t s = (base + 2 * j + 1) % NST;
                     if (!wait_all(edge + s, (phases >> s) & 1)) break;
                     phases ^= 1u << s;
-                    uint4* tile = reinterpret_cast<uint4*>(smem + L::kRing + s * L::kTile);
-                    uint32_t odd = 0;
+                    const int from = max(t.seen - j * kRows, 0);   // rows before it are seen by all
+#pragma unroll 1
+                    for (int slab = 0; slab < SLABS; ++slab) {
+                        uint4* tile = reinterpret_cast<uint4*>(smem + L::kRing + s * L::kTile + slab * SLAB);
+                        uint32_t odd = 0;
 #pragma unroll 8
-                    for (int e = (warp - 10) * 32 + lane; e < L::kTile / 16; e += 64) {
-                        const uint4 w = tile[e];
-                        odd |= not_finite<BF16>(w.x) | not_finite<BF16>(w.y) | not_finite<BF16>(w.z) | not_finite<BF16>(w.w);
-                    }
-                    if (__any_sync(NCM_FULL, odd)) {
-                        for (int e = (warp - 10) * 32 + lane; e < L::kTile / 16; e += 64) {
+                        for (int e = from * 8 + (warp - 10) * 32 + lane; e < kRows * 8; e += 64) {
+                            const uint4 w = tile[e];
+                            odd |= not_finite<BF16>(w.x) | not_finite<BF16>(w.y) | not_finite<BF16>(w.z) | not_finite<BF16>(w.w);
+                        }
+                        if (!__any_sync(NCM_FULL, odd)) continue;
+                        for (int e = from * 8 + (warp - 10) * 32 + lane; e < kRows * 8; e += 64) {
                             uint32_t* w = reinterpret_cast<uint32_t*>(tile + e);
                             for (int c = 0; c < 4; ++c) {
                                 const uint32_t bits = not_finite<BF16>(w[c]);
@@ -460,7 +482,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                         }
                         if (lane == 0) words[8 + (it & 7)] = it + 1;
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full + s);
@@ -475,7 +496,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // 32 lanes per warp, in bits 16 and up
         const uint32_t s_at = tmem + x * 128 + lanes, o_at = tmem + 256 + x * 128 + lanes;
         const int token = row / p.group, member = row % p.group;
-        uint32_t phases = 0, handed = 0;   // of s_ready; units given to the products
+        uint32_t phases = 0, used = 0, handed = 0;   // of s_ready, of o_ready; units given to the products
         for (int it = 0; ok; ++it) {
             const int index = item_index(it);
             if (it * (int)gridDim.x >= items) break;
@@ -520,7 +541,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                     if (over && now < INFINITY) top = now;
                     sum *= a;
                     if (!(now < INFINITY)) sum = NAN;
-                    if (u > 0) {   // O is at rest once the last unit's products are complete (those before it are: S of this unit is here)
+                    if (u > 0) {   // O is at rest once the last unit's products are complete (those before it are: S is here)
                         if (!wait_all(pv_done + x, (handed - 1) & 1)) break;
                         fence_after();
 #pragma unroll 1
@@ -566,14 +587,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 apart(l1, lc, ld);
                 sum += (la + lb) + (lc + ld);
             }
-            if (units > 0) {   // the last two units' products may both be on the way: one phase after the other
-                if (units > 1 && !wait_all(pv_done + x, handed & 1)) break;
-                if (!wait_all(pv_done + x, (handed - 1) & 1)) break;
+            if (units > 0) {
+                if (!wait_all(o_ready + x, used & 1)) break;
+                ++used;
                 fence_after();
             }
             const bool odd = words[8 + (it & 7)] == (uint32_t)(it + 1);
             const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;   // a row without keys: zeros
+            // Rows leave through shared memory, 32 columns at a time: four lanes then write 64
+            // bytes of a row, where one lane per row would touch 32 lines with every store.
             uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)(t.q0 + at) * p.out_stride + (int64_t)(t.head * p.group + member) * HD;
+            uint8_t* stage = smem + L::kStore + warp * 2048;
+            const uint32_t rows = __ballot_sync(NCM_FULL, mine);
+            uint16_t* dst[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                dst[i] = reinterpret_cast<uint16_t*>(__shfl_sync(NCM_FULL, reinterpret_cast<unsigned long long>(out), 8 * i + (lane >> 2))) + 8 * (lane & 3);
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
@@ -587,22 +616,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (odd && mine) {
                     // infinities and NaN that were taken out of V, for the rows that see their keys
                     const uint16_t* v = static_cast<const uint16_t*>(p.v) + (int64_t)t.k0 * p.v_stride + t.head * HD + c;
-                    for (int key = t.seen / kRows * kRows; key <= limit; ++key)
+                    for (int key = t.seen; key <= limit; ++key)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const uint16_t h = __ldg(v + key * p.v_stride + i);
                             if (not_finite<BF16>(h)) o[i] = __float_as_uint(__uint_as_float(o[i]) + widen<BF16>(h));
                         }
                 }
-                if (mine) {
+                __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint32_t w[4];
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = pack<BF16>(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-                        *reinterpret_cast<uint4*>(out + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = pack<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 8 * i + (lane >> 2);
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+                    if (rows >> r & 1) *reinterpret_cast<uint4*>(dst[i] + c) = w;
                 }
             }
             fence_before();   // O is read before the next item's products overwrite it
@@ -636,7 +671,7 @@ bool q_map(CUtensorMap* m, const void* base, int hd, int group, int kv_heads, in
 
 template <bool BF16, int HD>
 int prompt_run(const PromptParams& p, int grid, cudaStream_t s) {
-    const int bytes = Layout<BF16, HD>::kPrefix + 4 * (p.batch + 1);
+    const int bytes = Layout<BF16, HD>::kPrefix + 12 * (p.batch + 1);
     auto fn = prompt_attn_kernel<BF16, HD>;
     if (int r = set_smem_limit((const void*)fn, kPromptSmem)) return r;
     fn<<<grid, kPromptThreads, bytes, s>>>(p);
