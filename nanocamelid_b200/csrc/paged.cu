@@ -217,8 +217,17 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ attention of one token
 constexpr int kUnit = 32;              // keys that a warp takes at a time
-constexpr int kPagedWarps = 4;
-constexpr int kPagedBatch = 2048;      // sequences of one launch (their lengths lie in shared memory)
+#ifndef W128
+#define W128 6
+#define W64 8
+#define WQ1 8
+#define WQ2 8
+#endif
+#ifndef KPIECE
+#define KPIECE 4
+#endif
+constexpr int kPiece = KPIECE;              // units per warp up to which a segment stays in one CTA
+constexpr int kPagedBatch = 1024;      // sequences of one launch (their lengths lie in shared memory)
 constexpr int kPagedSmem = 232448;     // 227 KB
 
 struct alignas(64) PagedAttnParams {
@@ -230,7 +239,7 @@ struct alignas(64) PagedAttnParams {
     const int *lengths, *table;
     int table_width, batch, heads, kv_heads, group;
     int chunk, nchunk;                 // heads of a group that a segment takes, and segments per group
-    int log2ps, box_rows, nstages, min_share;
+    int log2ps, box_rows, nstages;
     int64_t pages;
     float scale_log2;
     float* part;                       // workspace: [2 * grid][chunk][hd] sums, then [2 * grid][chunk][2] (max, sum)
@@ -293,8 +302,11 @@ template <bool BF16> __device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
 }
 
 // A segment is one (sequence, key-value head, chunk of its query heads); its keys are cut in
-// units of 32, and all units of all segments lie in one row that is shared out evenly, first
-// over the CTAs, then over a CTA's warps.  A place in that row:
+// units of 32.  All units of all segments lie in one row that is shared out evenly, first
+// over the CTAs, then over a CTA's warps; when there are so few that every CTA can take at
+// most `kPiece` units per warp of a single segment, the row is padded so that no CTA has
+// two segments: a segment that fits one CTA is then joined in shared memory alone (a join
+// over CTAs costs about 4 us).  Positions fit 32 bits: the host sees to it.  A place in the row:
 struct Place {
     int b, hk, u, n;   // sequence, segment within it, unit within the segment, units of the segment
 };
@@ -307,8 +319,8 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, float4 v) {
 }
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : ex2(m - top); }
 
-template <bool BF16, bool Q8, int HD, int NT>
-__global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+template <bool BF16, bool Q8, int HD, int NT, int W>
+__global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     constexpr int GH = 8 * NT;                                   // head slots of a segment
     constexpr int KB = kUnit * HD * (Q8 ? 1 : 2);                // bytes of a unit's K (or V) values
@@ -319,93 +331,114 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
     const int nst = p.nstages;
 
     uint8_t* smem = smem_raw;                                    // ring [warp][stage][STAGE]
-    uint8_t* after = smem + (size_t)kPagedWarps * nst * STAGE;
+    uint8_t* after = smem + (size_t)W * nst * STAGE;
     float* first = reinterpret_cast<float*>(after);              // [warp][GH][HD], then [warp][GH][2]
-    float* first_ml = first + kPagedWarps * GH * HD;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(first_ml + kPagedWarps * GH * 2);   // [warp][stage][2]
-    int64_t* ent = reinterpret_cast<int64_t*>(bars + kPagedWarps * nst * 2);         // [8][3]: segment, begin, end
-    int* sums = reinterpret_cast<int*>(ent + 2 * kPagedWarps * 3);                   // [8]
-    int* prefix = sums + 8;                                      // [batch + 1]
+    float* first_ml = first + W * GH * HD;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(first_ml + W * GH * 2);   // [warp][stage][2]
+    int* ent = reinterpret_cast<int*>(bars + W * nst * 2);       // [2 W][4]: sequence (-1: none), segment, begin, end
+    int* sums = ent + 2 * W * 4;                                 // [2 W + 2]
+    int* prefix = sums + 2 * W + 2;                                      // [batch + 1]
     int* lens = prefix + p.batch + 1;                            // [batch]
 
-    // ---- lengths and their running sum of units
+    // ---- lengths and their running sum of units, as they are and padded to pieces
     const int HK = p.kv_heads * p.nchunk;
+    constexpr int PIECE = kPiece * W;
+    bool pieces;
     {
-        const int per = (p.batch + kPagedWarps * 32 - 1) / (kPagedWarps * 32);
+        const int per = (p.batch + W * 32 - 1) / (W * 32);
         const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-        int sum = 0;
-        const int64_t cap = (int64_t)p.table_width << p.log2ps;
+        int sum = 0, sum_p = 0;
+        const int cap = p.table_width << p.log2ps;
         for (int b = b0; b < b1; ++b) {
             int n = __ldg(p.lengths + b);
             if (n > cap) {
-                n = (int)cap;
+                n = cap;
                 if (blockIdx.x == 0) set_dev_error(p.err, NCM_DEVERR_BAD_ARG);
             }
             n = max(n, 0);
             lens[b] = n;
-            prefix[b + 1] = (n + kUnit - 1) / kUnit;
-            sum += prefix[b + 1];
+            sum += (n + kUnit - 1) / kUnit;
+            sum_p += (n + kUnit * PIECE - 1) / (kUnit * PIECE);
         }
-        int run = sum;
+        int run = sum, run_p = sum_p;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(NCM_FULL, run, o);
-            if (lane >= o) run += v;
+            const int v = __shfl_up_sync(NCM_FULL, run, o), v_p = __shfl_up_sync(NCM_FULL, run_p, o);
+            if (lane >= o) { run += v; run_p += v_p; }
         }
-        if (lane == 31) sums[warp] = run;
-        if (tid < 2 * kPagedWarps) ent[3 * tid] = -1;
+        if (lane == 31) { sums[2 * warp] = run; sums[2 * warp + 1] = run_p; }
+        if (tid < 2 * W) ent[4 * tid] = -1;
         if (lane == 0)
             for (int i = 0; i < 2 * nst; ++i) mbar_init(bars + warp * nst * 2 + i, 1);
         fence_mbar_init();
         __syncthreads();
         run -= sum;
-        for (int w = 0; w < warp; ++w) run += sums[w];
+        run_p -= sum_p;
+        int all_p = 0;
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) { run += sums[2 * w]; run_p += sums[2 * w + 1]; }
+            all_p += sums[2 * w + 1];
+        }
+        pieces = all_p <= (int)gridDim.x / HK;
         if (tid == 0) prefix[0] = 0;
-        for (int b = b0; b < b1; ++b) { run += prefix[b + 1]; prefix[b + 1] = run; }
+        for (int b = b0; b < b1; ++b) {
+            if (pieces) {
+                run_p += (lens[b] + kUnit * PIECE - 1) / (kUnit * PIECE);
+                prefix[b + 1] = run_p * PIECE;
+            } else {
+                run += (lens[b] + kUnit - 1) / kUnit;
+                prefix[b + 1] = run;
+            }
+        }
         __syncthreads();
     }
     // rows of sequences without keys
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
         if (lens[b] == 0)
-            for (int i = 4 * tid; i < p.heads * HD; i += 4 * kPagedWarps * 32)
+            for (int i = 4 * tid; i < p.heads * HD; i += 4 * W * 32)
                 store_out<BF16>(p.out, b * p.out_stride + i, make_float4(0.f, 0.f, 0.f, 0.f));
 
-    const int64_t total = (int64_t)prefix[p.batch] * HK;
-    const int64_t share = max((int64_t)p.min_share, (total + gridDim.x - 1) / gridDim.x);
-    const int64_t u0 = min(total, blockIdx.x * share), u1 = min(total, u0 + share);
-    if (u0 >= u1) return;
-    const int per_warp = (int)((u1 - u0 + kPagedWarps - 1) / kPagedWarps);
-    const int64_t w0 = min(u1, u0 + (int64_t)warp * per_warp), w1 = min(u1, w0 + per_warp);
-    const int count = (int)(w1 - w0);
+    const int total = prefix[p.batch] * HK;
+    const int share = pieces ? PIECE : max(PIECE, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int u0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
+    if (u0 >= total) return;
+    Place c;
+    auto find = [&](int at) {   // the place at this position of the row
+        int lo = 0, hi = p.batch;   // last b with prefix[b] * HK <= at
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] * HK <= at) lo = mid; else hi = mid;
+        }
+        const int stride = prefix[lo + 1] - prefix[lo], rest = at - prefix[lo] * HK;
+        c.b = lo;
+        c.n = (lens[lo] + kUnit - 1) / kUnit;
+        c.hk = rest / stride;
+        c.u = rest - c.hk * stride;
+    };
+    find(u0);
+    const int u1 = pieces ? u0 + min(share, c.n - c.u) : (int)min((int64_t)total, (int64_t)u0 + share);
+    const int per_warp = (u1 - u0 + W - 1) / W;
+    const int w0 = min(u1, u0 + warp * per_warp), w1 = min(u1, w0 + per_warp);
+    const int count = w1 - w0;
+    if (count > 0) {
+        if (pieces) c.u += w0 - u0; else find(w0);
+    }
 
     // ---- this warp's units
     uint8_t* ring = smem + (size_t)warp * nst * STAGE;
     uint64_t* bar = bars + warp * nst * 2;
-    Place c;
-    {
-        int lo = 0, hi = p.batch;   // last b with prefix[b] * HK <= w0
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((int64_t)prefix[mid] * HK <= w0) lo = mid; else hi = mid;
-        }
-        c.b = lo;
-        c.n = prefix[lo + 1] - prefix[lo];
-        const int64_t rest = w0 - (int64_t)prefix[lo] * HK;
-        c.hk = c.n ? (int)(rest / c.n) : 0;
-        c.u = c.n ? (int)(rest % c.n) : 0;
-    }
     auto next = [&](Place& t) {
         if (++t.u < t.n) return;
         t.u = 0;
         if (++t.hk < HK) return;
         t.hk = 0;
-        do { ++t.b; } while (t.b < p.batch && prefix[t.b + 1] == prefix[t.b]);
-        t.n = t.b < p.batch ? prefix[t.b + 1] - prefix[t.b] : 1;
+        do { ++t.b; } while (t.b < p.batch && lens[t.b] == 0);
+        t.n = t.b < p.batch ? (lens[t.b] + kUnit - 1) / kUnit : 1;
     };
     const int box = p.box_rows, lbox = 31 - __clz(box), npg = kUnit / box;   // boxes of a unit: one per page, or one of 32 rows
-    auto page_of = [&](const Place& t) -> int {      // lane i < npg: the page of box i
-        const int key = t.u * kUnit + lane * box;
-        if (lane >= npg || key >= lens[t.b]) return -1;
+    auto page_at = [&](const Place& t, int i) -> int {   // the page of box i < npg
+        const int key = t.u * kUnit + i * box;
+        if (i >= npg || key >= lens[t.b]) return -1;
         const int id = __ldg(p.table + (int64_t)t.b * p.table_width + (key >> p.log2ps));
         if (id < 0 || id >= p.pages) set_dev_error(p.err, NCM_DEVERR_BAD_ARG);   // TMA reads zeros there
         return id;
@@ -424,26 +457,17 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
         __syncwarp();
         if (mine) {
             const int row = key & ((1 << p.log2ps) - 1), h = t.hk / p.nchunk;
-            constexpr int W = Q8 ? HD : 128;   // bytes of a swizzled row
+            constexpr int ROW = Q8 ? HD : 128;   // bytes of a swizzled row
 #pragma unroll
-            for (int j = 0; j < KB / (kUnit * W); ++j)
-                tma_load_4d(st + j * kUnit * W + lane * box * W, &p.km, kb, j * 64, row, h, page);
+            for (int j = 0; j < KB / (kUnit * ROW); ++j)
+                tma_load_4d(st + j * kUnit * ROW + lane * box * ROW, &p.km, kb, j * 64, row, h, page);
             if (Q8) tma_load_3d(st + 2 * KB + lane * 128, &p.ksm, kb, row * NB, h, page);
 #pragma unroll
-            for (int j = 0; j < KB / (kUnit * W); ++j)
-                tma_load_4d(st + KB + j * kUnit * W + lane * box * W, &p.vm, kb + 1, j * 64, row, h, page);
+            for (int j = 0; j < KB / (kUnit * ROW); ++j)
+                tma_load_4d(st + KB + j * kUnit * ROW + lane * box * ROW, &p.vm, kb + 1, j * 64, row, h, page);
             if (Q8) tma_load_3d(st + 2 * KB + SB + lane * 128, &p.vsm, kb + 1, row * NB, h, page);
         }
     };
-    Place f = c;                  // the next unit to be fetched, and its pages
-    int fetched = 0, fpage = 0;
-    if (count > 0) fpage = page_of(f);
-    for (; fetched < min(count, nst); ++fetched) {
-        issue(f, fpage, fetched);
-        next(f);
-        if (fetched + 1 < count) fpage = page_of(f);
-    }
-
     uint32_t qf[KS][NT][2];
     float o[KS][NT][4], m[NT][2], l[NT][2];
     auto begin = [&]() {          // the segment's queries, and empty sums
@@ -491,6 +515,29 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
     int began = 0;                // first unit (of this warp) of the current segment
     bool failed = false;
     if (count > 0) begin();
+    Place f = c;                  // the next unit to be fetched, and its pages
+    int fetched = 0, fpage = 0;
+    {
+        // The first units' pages by one load: lane i of the unit i / npg.  The loads of the
+        // queries above are on their way meanwhile.
+        const int most = min(min(count, nst), 32 / npg), mine = lane / npg;
+        int page = 0;
+        if (mine < most) {
+            Place t = c;
+            for (int i = 0; i < mine; ++i) next(t);
+            page = page_at(t, lane % npg);
+        }
+        for (; fetched < most; ++fetched) {
+            issue(f, __shfl_sync(NCM_FULL, page, (fetched * npg + lane) & 31), fetched);
+            next(f);
+        }
+        if (fetched < count) fpage = page_at(f, lane);
+        for (; fetched < min(count, nst); ++fetched) {
+            issue(f, fpage, fetched);
+            next(f);
+            if (fetched + 1 < count) fpage = page_at(f, lane);
+        }
+    }
     for (int i = 0, stage = 0, phase = 0; i < count && !failed; ++i) {
         uint8_t* st = ring + stage * STAGE;
         const uint32_t ka = smem_u32(st), va = ka + KB;
@@ -596,12 +643,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
             }
         if (!mbar_wait(bar + 2 * stage + 1, phase, kPagedWaitNs)) { failed = true; break; }
         if (valid < kUnit) {   // rows behind the last key may hold anything: zero x NaN is NaN
-            constexpr int W = Q8 ? HD : 128;
-            for (int e = lane; e < (kUnit - valid) * (W / 16); e += 32) {
-                const int row = valid + e / (W / 16);
+            constexpr int ROW = Q8 ? HD : 128;
+            for (int e = lane; e < (kUnit - valid) * (ROW / 16); e += 32) {
+                const int row = valid + e / (ROW / 16);
 #pragma unroll
-                for (int j = 0; j < KB / (kUnit * W); ++j)
-                    *reinterpret_cast<uint4*>(st + KB + j * kUnit * W + row * W + (e % (W / 16)) * 16) = make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < KB / (kUnit * ROW); ++j)
+                    *reinterpret_cast<uint4*>(st + KB + j * kUnit * ROW + row * ROW + (e % (ROW / 16)) * 16) = make_uint4(0, 0, 0, 0);
             }
             if (Q8)
                 for (int e = lane; e < (kUnit - valid) * NB; e += 32) vsc[scale_at(valid + e / NB) + e % NB] = __half(0.0f);
@@ -668,7 +715,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
         if (fetched < count) {
             issue(f, fpage, stage);
             next(f);
-            if (++fetched < count) fpage = page_of(f);
+            if (++fetched < count) fpage = page_at(f, lane);
         }
         if (++stage == nst) { stage = 0; phase ^= 1; }
 
@@ -693,10 +740,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
                     }
             } else {
                 const bool at_end = i + 1 == count;
-                int64_t* e = ent + 3 * (2 * warp + (at_end ? 1 : 0));
+                int* e = ent + 4 * (2 * warp + (at_end ? 1 : 0));
                 if (lane == 0) {
-                    const int64_t base = (int64_t)prefix[c.b] * HK + (int64_t)c.hk * c.n;
-                    e[0] = (int64_t)c.b * HK + c.hk; e[1] = base; e[2] = base + c.n;
+                    const int base = prefix[c.b] * HK + c.hk * (prefix[c.b + 1] - prefix[c.b]);
+                    e[0] = c.b; e[1] = c.hk; e[2] = base; e[3] = base + c.n;
                 }
                 if (!at_end) keep(first + warp * GH * HD, first_ml + warp * GH * 2);
             }
@@ -713,33 +760,40 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
     }
     __syncthreads();   // every copy has landed: the ring holds the warps' last parts now
     float* last = reinterpret_cast<float*>(smem);
-    float* last_ml = last + kPagedWarps * GH * HD;
-    if (count > 0 && ent[3 * (2 * warp + 1)] >= 0) keep(last + warp * GH * HD, last_ml + warp * GH * 2);
+    float* last_ml = last + W * GH * HD;
+    if (count > 0 && ent[4 * (2 * warp + 1)] >= 0) keep(last + warp * GH * HD, last_ml + warp * GH * 2);
     __syncthreads();
 
     // ---- the CTA's parts, joined where they are of one segment
-    float* weights = last_ml + kPagedWarps * GH * 2;   // [parts][GH] of the join over CTAs
-    for (int e = 0; e < 2 * kPagedWarps;) {
-        const int64_t seg = ent[3 * e];
-        if (seg < 0) { ++e; continue; }
-        const int64_t sb = ent[3 * e + 1], se = ent[3 * e + 2];
-        int e1 = e + 1;
-        while (e1 < 2 * kPagedWarps && (ent[3 * e1] < 0 || ent[3 * e1] == seg)) ++e1;
-        const int b = (int)(seg / HK), hk = (int)(seg % HK), h = hk / p.nchunk, ch = hk % p.nchunk;
+    float* weights = last_ml + W * GH * 2;   // [parts][GH] of the join over CTAs
+    for (int e = 0; e < 2 * W;) {
+        const int4 seg = *reinterpret_cast<const int4*>(ent + 4 * e);
+        if (seg.x < 0) { ++e; continue; }
+        const int b = seg.x, hk = seg.y, sb = seg.z, se = seg.w, h = hk / p.nchunk, ch = hk - h * p.nchunk;
+        uint32_t of = 0;   // the entries of this segment: those up to the next one's first
+        int e1 = e;
+        for (; e1 < 2 * W; ++e1) {
+            const int4 o = *reinterpret_cast<const int4*>(ent + 4 * e1);
+            if (o.x < 0) continue;
+            if (o.x != b || o.y != hk) break;
+            of |= 1u << e1;
+        }
         const int heads = min(p.chunk, p.group - ch * p.chunk);
         const int64_t out_at = b * p.out_stride + (int64_t)(h * p.group + ch * p.chunk) * HD;
         const bool inside = sb >= u0 && se <= u1;
         const int slot = sb < u0 ? 0 : 1;
         float* rows = p.part + (int64_t)(2 * blockIdx.x + slot) * p.chunk * HD;
         float* mls = p.part + (int64_t)2 * gridDim.x * p.chunk * HD;
-        for (int x = tid; x < heads * (HD / 4); x += kPagedWarps * 32) {
+        for (int x = tid; x < heads * (HD / 4); x += W * 32) {
             const int head = x / (HD / 4), d = 4 * (x % (HD / 4));
             float top = -INFINITY, sum = 0.0f;
-            for (int y = e; y < e1; ++y)
-                if (ent[3 * y] == seg) top = fmaxf(top, ((y & 1) ? last_ml : first_ml)[((y >> 1) * GH + head) * 2]);
+#pragma unroll
+            for (int y = 0; y < 2 * W; ++y)
+                if (of >> y & 1) top = fmaxf(top, ((y & 1) ? last_ml : first_ml)[((y >> 1) * GH + head) * 2]);
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int y = e; y < e1; ++y) {
-                if (ent[3 * y] != seg) continue;
+#pragma unroll
+            for (int y = 0; y < 2 * W; ++y) {
+                if (!(of >> y & 1)) continue;
                 const float* ml = ((y & 1) ? last_ml : first_ml) + ((y >> 1) * GH + head) * 2;
                 const float4 v = *reinterpret_cast<const float4*>(((y & 1) ? last : first) + ((y >> 1) * GH + head) * HD + d);
                 const float w = part_weight(ml[0], top);
@@ -761,20 +815,49 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
         if (!inside) {
             // The CTA that stores its part last joins them all, in the CTAs' order: the result
             // does not depend on which one that is.  Nobody waits.
-            const int i0 = (int)(sb / share), i1 = (int)((se - 1) / share);
+            const int i0 = sb / share, i1 = (se - 1) / share;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                sums[4] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
-                if (sums[4]) p.counters[i0] = 0;
+                sums[2 * W] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
+                if (sums[2 * W]) p.counters[i0] = 0;
             }
             __syncthreads();
-            if (sums[4]) {
+            if (sums[2 * W]) {
                 __threadfence();
                 const int np = i1 - i0 + 1;
                 auto part_of = [&](int i) { return (int64_t)(2 * (i0 + i) + (i == 0 ? 1 : 0)); };
+                if (np <= 8) {   // one round of loads
+                    for (int x = tid; x < heads * (HD / 4); x += W * 32) {
+                        const int head = x / (HD / 4), d = 4 * (x % (HD / 4));
+                        float2 ml[8];
+                        float4 v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int64_t at = part_of(min(i, np - 1)) * p.chunk + head;
+                            ml[i] = __ldcg(reinterpret_cast<const float2*>(mls + at * 2));
+                            v[i] = __ldcg(reinterpret_cast<const float4*>(p.part + at * HD + d));
+                        }
+                        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if (i >= np) break;
+                            const float w = part_weight(ml[i].x, top);
+                            acc.x = fmaf(w, v[i].x, acc.x); acc.y = fmaf(w, v[i].y, acc.y);
+                            acc.z = fmaf(w, v[i].z, acc.z); acc.w = fmaf(w, v[i].w, acc.w);
+                            sum = fmaf(w, ml[i].y, sum);
+                        }
+                        const float inv = 1.0f / sum;
+                        store_out<BF16>(p.out, out_at + head * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+                    }
+                    e = e1;
+                    continue;
+                }
                 // weights of the parts, one warp per head in turn; their joint sum is folded in
-                for (int head = warp; head < heads; head += kPagedWarps) {
+                for (int head = warp; head < heads; head += W) {
                     float top = -INFINITY, sum = 0.0f;
                     for (int i = lane; i < np; i += 32) top = fmaxf(top, __ldcg(mls + (part_of(i) * p.chunk + head) * 2));
 #pragma unroll
@@ -791,7 +874,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) paged_attn_kernel(const _
                     for (int i = lane; i < np; i += 32) weights[i * GH + head] *= inv;
                 }
                 __syncthreads();
-                for (int x = tid; x < heads * (HD / 4); x += kPagedWarps * 32) {
+                for (int x = tid; x < heads * (HD / 4); x += W * 32) {
                     const int head = x / (HD / 4), d = 4 * (x % (HD / 4));
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
@@ -874,23 +957,24 @@ int paged_maps(const ncm_paged_kv* kv, int box, PagedAttnParams& p) {
     return 0;
 }
 
-template <bool BF16, bool Q8, int HD, int NT>
+template <bool BF16, bool Q8, int HD, int NT, int W>
 int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
     const int stage = 2 * (kUnit * HD * (Q8 ? 1 : 2) + (Q8 ? 512 : 0));
-    const int fixed = kPagedWarps * 8 * NT * (HD + 2) * 4 + 2 * kPagedWarps * 3 * 8 + 32 + (2 * p.batch + 1) * 4;
+    const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (2 * W + 2) * 4 + (2 * p.batch + 1) * 4;
     int n = 1;   // stages: as many as fit, 8 at most
-    while (n < 8 && fixed + kPagedWarps * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
+    while (n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
     p.nstages = n;
-    auto fn = paged_attn_kernel<BF16, Q8, HD, NT>;
+    auto fn = paged_attn_kernel<BF16, Q8, HD, NT, W>;
     if (int r = set_smem_limit((const void*)fn, kPagedSmem)) return r;
-    fn<<<grid, kPagedWarps * 32, fixed + kPagedWarps * n * (stage + 16), s>>>(p);
+    fn<<<grid, W * 32, fixed + W * n * (stage + 16), s>>>(p);
     return (int)cudaGetLastError();
 }
 template <bool BF16, bool Q8>
 int paged_attn_pick(PagedAttnParams& p, int hd, int grid, cudaStream_t s) {
     const bool two = p.chunk > 8;
-    if (hd == 64) return two ? paged_attn_run<BF16, Q8, 64, 2>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1>(p, grid, s);
-    return two ? paged_attn_run<BF16, Q8, 128, 2>(p, grid, s) : paged_attn_run<BF16, Q8, 128, 1>(p, grid, s);
+    if (hd == 64) return two ? paged_attn_run<BF16, Q8, 64, 2, W64>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1, W64>(p, grid, s);
+    if (two) return paged_attn_run<BF16, Q8, 128, 2, Q8 ? WQ2 : 4>(p, grid, s);
+    return paged_attn_run<BF16, Q8, 128, 1, Q8 ? WQ1 : W128>(p, grid, s);
 }
 
 int bad(const char* what) { return set_error(NCM_EINVAL, what); }
@@ -1000,11 +1084,14 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)hd)) * 1.4426950408889634f;
     p.counters = (unsigned*)workspace;
     p.part = (float*)((char*)workspace + 4096);
-    p.min_share = 2 * kPagedWarps;
     p.err = err;
+    // positions in the row of units, padded to pieces, fit 32 bits
+    const int64_t most = ((int64_t)table_width * kv->page_size / (kUnit * kPiece * 8) + 1) * kPiece * 8 * kv->kv_heads * p.nchunk;
+    const int step = (int)std::min<int64_t>(kPagedBatch, (int64_t)0x7fff0000 / most);
+    if (step < 1) return set_error(NCM_EUNSUPPORTED, "a sequence's pages hold too many tokens for so many heads");
     cudaStream_t s = (cudaStream_t)stream;
-    for (int b = 0; b < batch; b += kPagedBatch) {
-        p.batch = std::min(kPagedBatch, batch - b);
+    for (int b = 0; b < batch; b += step) {
+        p.batch = std::min(step, batch - b);
         p.q = (const uint16_t*)q + b * q_stride;
         p.out = (uint16_t*)out + b * out_stride;
         p.lengths = lengths + b;
