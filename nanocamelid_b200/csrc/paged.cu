@@ -217,16 +217,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ attention of one token
 constexpr int kUnit = 32;              // keys that a warp takes at a time
-#ifndef W128
-#define W128 6
-#define W64 8
-#define WQ1 8
-#define WQ2 8
-#endif
-#ifndef KPIECE
-#define KPIECE 4
-#endif
-constexpr int kPiece = KPIECE;              // units per warp up to which a segment stays in one CTA
+constexpr int kPiece = 8;              // units per warp up to which a segment stays in one CTA
 constexpr int kPagedBatch = 1024;      // sequences of one launch (their lengths lie in shared memory)
 constexpr int kPagedSmem = 232448;     // 227 KB
 
@@ -267,17 +258,17 @@ __device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t addr) {
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     if (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -285,20 +276,31 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two int8 in the low bytes of w's halves, as 16-bit floats, exactly: low seven bits and sign
-// bit are each or-ed under an exponent whose step is one, and subtracted.
-template <bool BF16> __device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
-    constexpr uint32_t base = BF16 ? 0x43004300u : 0x64006400u;
-    const uint32_t a = (w & 0x007f007fu) | base, b = (w & 0x00800080u) | base;
-    uint32_t r;
-    if (BF16) {
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-        r = *reinterpret_cast<const uint32_t*>(&d);
-    } else {
-        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-        r = *reinterpret_cast<const uint32_t*>(&d);
-    }
+// Integer products of int8 rows A with int8 (or unsigned) columns B, 32 deep.  The sum starts
+// from the bits of 1.5 * 2^23, so that the result is the float 1.5 * 2^23 + sum while |sum| < 2^22.
+constexpr uint32_t kIntBase = 0x4b400000u;
+constexpr float kIntBaseF = 12582912.0f;
+template <bool UNSIGNED_B>
+__device__ __forceinline__ void imma16832(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    uint32_t r0, r1, r2, r3;
+    if (UNSIGNED_B)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kIntBase));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kIntBase));
+    d[0] = __uint_as_float(r0); d[1] = __uint_as_float(r1); d[2] = __uint_as_float(r2); d[3] = __uint_as_float(r3);
+}
+// 256 hi + lo of two such results.
+__device__ __forceinline__ float joined(float hi, float lo) { return fmaf(hi - kIntBaseF, 256.0f, lo - kIntBaseF); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
+}
+template <bool BF16> __device__ __forceinline__ float2 widen2(uint32_t w) {
+    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 // A segment is one (sequence, key-value head, chunk of its query heads); its keys are cut in
@@ -319,6 +321,15 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, float4 v) {
 }
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : ex2(m - top); }
 
+__host__ __device__ constexpr bool one_stage(int hd, int nt) { return hd == 128 && nt == 1; }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(NCM_FULL, v, 0); }
+// One lane of a converged warp, in a form that the compiler knows for one.
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(yes));
+    return yes != 0;
+}
+
 template <bool BF16, bool Q8, int HD, int NT, int W>
 __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -327,6 +338,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     constexpr int SB = Q8 ? 512 : 0;                             // ... and of its scales
     constexpr int STAGE = 2 * (KB + SB);
     constexpr int KS = HD / 16, NB = HD / 32;
+    constexpr bool ONE = one_stage(HD, NT);                      // K and V of a unit are then fetched apart
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c4 = lane & 3, r8 = lane >> 2;
     const int nst = p.nstages;
 
@@ -435,7 +447,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         do { ++t.b; } while (t.b < p.batch && lens[t.b] == 0);
         t.n = t.b < p.batch ? (lens[t.b] + kUnit - 1) / kUnit : 1;
     };
-    const int box = p.box_rows, lbox = 31 - __clz(box), npg = kUnit / box;   // boxes of a unit: one per page, or one of 32 rows
+    const int box = p.box_rows, lbox = 31 - __clz(box), lnpg = 5 - lbox, npg = 1 << lnpg;   // boxes of a unit: one per page, or one of 32 rows
     auto page_at = [&](const Place& t, int i) -> int {   // the page of box i < npg
         const int key = t.u * kUnit + i * box;
         if (i >= npg || key >= lens[t.b]) return -1;
@@ -443,50 +455,98 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         if (id < 0 || id >= p.pages) set_dev_error(p.err, NCM_DEVERR_BAD_ARG);   // TMA reads zeros there
         return id;
     };
-    auto issue = [&](const Place& t, int page, int stage) {
-        const int key = t.u * kUnit + lane * box;
-        const bool mine = lane < npg && key < lens[t.b];
-        const int boxes = __popc(__ballot_sync(NCM_FULL, mine));
+    auto head_of = [&](int hk) { return p.nchunk == 1 ? hk : hk / p.nchunk; };
+    // Fetches a unit (with one stage its K or its V, since K's place is free before the softmax)
+    // whose boxes' pages lie in lanes 0 to npg - 1.  One lane issues, from uniform values: copies
+    // issued by the lanes that hold the pages took about 1000 cycles a unit.
+    auto issue = [&](const Place& t, int page, int stage, bool key_rows, bool value_rows) {
+        const int key = uniform(t.u * kUnit), h = uniform(head_of(t.hk));
+        const int boxes = min(npg, uniform((lens[t.b] - key + box - 1) >> lbox));
         uint8_t* st = ring + stage * STAGE;
         uint64_t* kb = bar + 2 * stage;
-        if (lane == 0) {
-            const uint32_t bytes = boxes * box * (HD * (Q8 ? 1 : 2) + (Q8 ? NB * 2 : 0));
-            mbar_arrive_expect_tx(kb, bytes);
-            mbar_arrive_expect_tx(kb + 1, bytes);
+        const uint32_t bytes = boxes * box * (HD * (Q8 ? 1 : 2) + (Q8 ? NB * 2 : 0));
+        if (elected()) {
+            if (key_rows) mbar_arrive_expect_tx(kb, bytes);
+            if (value_rows) mbar_arrive_expect_tx(kb + 1, bytes);
         }
-        __syncwarp();
-        if (mine) {
-            const int row = key & ((1 << p.log2ps) - 1), h = t.hk / p.nchunk;
-            constexpr int ROW = Q8 ? HD : 128;   // bytes of a swizzled row
+        constexpr int ROW = Q8 ? HD : 128;   // bytes of a swizzled row
+#pragma unroll 1
+        for (int i = 0; i < boxes; ++i) {
+            const int id = __shfl_sync(NCM_FULL, page, i), row = (key + i * box) & ((1 << p.log2ps) - 1);
+            if (elected()) {
+                if (key_rows) {
 #pragma unroll
-            for (int j = 0; j < KB / (kUnit * ROW); ++j)
-                tma_load_4d(st + j * kUnit * ROW + lane * box * ROW, &p.km, kb, j * 64, row, h, page);
-            if (Q8) tma_load_3d(st + 2 * KB + lane * 128, &p.ksm, kb, row * NB, h, page);
+                    for (int j = 0; j < KB / (kUnit * ROW); ++j)
+                        tma_load_4d(st + j * kUnit * ROW + i * box * ROW, &p.km, kb, j * 64, row, h, id);
+                    if (Q8) tma_load_3d(st + 2 * KB + i * 128, &p.ksm, kb, row * NB, h, id);
+                }
+                if (value_rows) {
 #pragma unroll
-            for (int j = 0; j < KB / (kUnit * ROW); ++j)
-                tma_load_4d(st + KB + j * kUnit * ROW + lane * box * ROW, &p.vm, kb + 1, j * 64, row, h, page);
-            if (Q8) tma_load_3d(st + 2 * KB + SB + lane * 128, &p.vsm, kb + 1, row * NB, h, page);
+                    for (int j = 0; j < KB / (kUnit * ROW); ++j)
+                        tma_load_4d(st + KB + j * kUnit * ROW + i * box * ROW, &p.vm, kb + 1, j * 64, row, h, id);
+                    if (Q8) tma_load_3d(st + 2 * KB + SB + i * 128, &p.vsm, kb + 1, row * NB, h, id);
+                }
+            }
+            __syncwarp();
         }
     };
+    // Queries: 16-bit values as they are; over Q8_0 as 16-bit integers per block of 32 (high bytes in
+    // qf[2 k], low bytes in qf[2 k + 1]), whose scales qs belong to this lane's two heads of the products.
     uint32_t qf[KS][NT][2];
+    float qs[NB][NT][2];
     float o[KS][NT][4], m[NT][2], l[NT][2];
     auto begin = [&]() {          // the segment's queries, and empty sums
-        const int h = c.hk / p.nchunk, ch = c.hk % p.nchunk;
+        const int h = head_of(c.hk), ch = c.hk - h * p.nchunk;
         const int heads = min(p.chunk, p.group - ch * p.chunk);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int head = t * 8 + r8;
             const uint16_t* q = static_cast<const uint16_t*>(p.q) + c.b * p.q_stride +
                                 (int64_t)(h * p.group + ch * p.chunk + head) * HD;
+            if (!Q8) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                // Q8_0: a lane's four neighbouring bytes of K are its four columns of the product
-                const int d0 = s * 16 + (Q8 ? 4 * c4 : 2 * c4), d1 = d0 + (Q8 ? 2 : 8);
-                qf[s][t][0] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + d0)) : 0u;
-                qf[s][t][1] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + d1)) : 0u;
+                for (int s = 0; s < KS; ++s) {
+                    qf[s][t][0] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + s * 16 + 2 * c4)) : 0u;
+                    qf[s][t][1] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + s * 16 + 8 + 2 * c4)) : 0u;
+                }
+            } else {
+                uint2 raw[NB][2];   // d = 32 k + 16 i + 4 c4 + 0..3
+#pragma unroll
+                for (int k = 0; k < NB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        raw[k][i] = head < heads ? __ldg(reinterpret_cast<const uint2*>(q + 32 * k + 16 * i + 4 * c4)) : make_uint2(0, 0);
+#pragma unroll
+                for (int k = 0; k < NB; ++k) {
+                    float x[8], top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 f0 = widen2<BF16>(raw[k][i].x), f1 = widen2<BF16>(raw[k][i].y);
+                        x[4 * i] = f0.x; x[4 * i + 1] = f0.y; x[4 * i + 2] = f1.x; x[4 * i + 3] = f1.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+                    top = max_nan(top, __shfl_xor_sync(NCM_FULL, top, 1));
+                    top = max_nan(top, __shfl_xor_sync(NCM_FULL, top, 2));
+                    const float inv = top > 0.0f && top < INFINITY ? 32512.0f / top : 0.0f;   // 127 * 256: high bytes fit
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[4 * i + e], inv, kIntBaseF));   // low 16 bits
+                        const uint32_t v01 = __byte_perm(v[0], v[1], 0x5410), v23 = __byte_perm(v[2], v[3], 0x5410);
+                        qf[2 * k][t][i] = __byte_perm(v01, v23, 0x7531);
+                        qf[2 * k + 1][t][i] = __byte_perm(v01, v23, 0x6420);
+                    }
+                    const float sc = top < INFINITY ? top * (1.0f / 32512.0f) : NAN;   // a query that is not finite: NaN
+                    qs[k][t][0] = __shfl_sync(NCM_FULL, sc, 8 * c4);
+                    qs[k][t][1] = __shfl_sync(NCM_FULL, sc, 8 * c4 + 4);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[s][t][i] = 0.0f;
-            }
             m[t][0] = m[t][1] = -INFINITY;
             l[t][0] = l[t][1] = 0.0f;
         }
@@ -520,23 +580,19 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     {
         // The first units' pages by one load: lane i of the unit i / npg.  The loads of the
         // queries above are on their way meanwhile.
-        const int most = min(min(count, nst), 32 / npg), mine = lane / npg;
+        const int most = min(count, nst), mine = lane >> lnpg;   // 8 units of 4 boxes at most
         int page = 0;
         if (mine < most) {
             Place t = c;
             for (int i = 0; i < mine; ++i) next(t);
-            page = page_at(t, lane % npg);
+            page = page_at(t, lane & (npg - 1));
         }
+        __syncwarp();
         for (; fetched < most; ++fetched) {
-            issue(f, __shfl_sync(NCM_FULL, page, (fetched * npg + lane) & 31), fetched);
+            issue(f, __shfl_sync(NCM_FULL, page, ((fetched << lnpg) + lane) & 31), fetched, true, true);
             next(f);
         }
         if (fetched < count) fpage = page_at(f, lane);
-        for (; fetched < min(count, nst); ++fetched) {
-            issue(f, fpage, fetched);
-            next(f);
-            if (fetched + 1 < count) fpage = page_at(f, lane);
-        }
     }
     for (int i = 0, stage = 0, phase = 0; i < count && !failed; ++i) {
         uint8_t* st = ring + stage * STAGE;
@@ -546,6 +602,21 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         const int valid = lens[c.b] - c.u * kUnit;   // keys of this unit (32 or more: all)
         // scale rows lie 128 bytes apart per box when a box has few rows
         auto scale_at = [&](int row) { return (row >> lbox) * 64 + (row & (box - 1)) * NB; };
+        // the scales of this lane's four rows
+        auto scales_of = [&](const __half* at, float (*to)[NB]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[NB / 2];
+                const __half* row = at + scale_at(r8 + 8 * i);
+                if (NB == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(row);
+                else w[0] = *reinterpret_cast<const uint32_t*>(row);
+#pragma unroll
+                for (int k = 0; k < NB / 2; ++k) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                    to[i][2 * k] = f.x; to[i][2 * k + 1] = f.y;
+                }
+            }
+        };
         if (!mbar_wait(bar + 2 * stage, phase, kPagedWaitNs)) { failed = true; break; }
         // scores: rows = keys, columns = heads
         float s[2][NT][4];
@@ -570,6 +641,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         } else {
             const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
             const int swz = HD == 128 ? (row & 7) : ((row >> 1) & 3);
+            float sk[4][NB];
+            scales_of(ksc, sk);
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -577,20 +650,14 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     const int col = 2 * k + (lane >> 4);
                     uint32_t x[4];
                     ldsm4(x, ka + (a * 16 + row) * HD + ((col ^ swz) << 4));
-                    const float s0 = __half2float(ksc[scale_at(a * 16 + r8) + k]);
-                    const float s1 = __half2float(ksc[scale_at(a * 16 + r8 + 8) + k]);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
+                        float hi[4], lo[4];
+                        imma16832<false>(hi, x[0], x[1], x[2], x[3], qf[2 * k][t][0], qf[2 * k][t][1]);
+                        imma16832<true>(lo, x[0], x[1], x[2], x[3], qf[2 * k + 1][t][0], qf[2 * k + 1][t][1]);
 #pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                            mma16816<BF16>(d, int8_pair<BF16>(__byte_perm(x[2 * g], 0, 0x4140)),
-                                           int8_pair<BF16>(__byte_perm(x[2 * g + 1], 0, 0x4140)),
-                                           int8_pair<BF16>(__byte_perm(x[2 * g], 0, 0x4342)),
-                                           int8_pair<BF16>(__byte_perm(x[2 * g + 1], 0, 0x4342)), qf[2 * k + g][t][0],
-                                           qf[2 * k + g][t][1]);
-                        s[a][t][0] = fmaf(s0, d[0], s[a][t][0]); s[a][t][1] = fmaf(s0, d[1], s[a][t][1]);
-                        s[a][t][2] = fmaf(s1, d[2], s[a][t][2]); s[a][t][3] = fmaf(s1, d[3], s[a][t][3]);
+                        for (int j = 0; j < 4; ++j)
+                            s[a][t][j] = fmaf(joined(hi[j], lo[j]), sk[2 * a + (j >> 1)][k] * qs[k][t][j & 1], s[a][t][j]);
                     }
                 }
         }
@@ -630,6 +697,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     for (int k = 0; k < KS; ++k) { o[k][t][j] *= a; o[k][t][j + 2] *= a; }
                 }
         }
+        if (ONE && fetched < count) issue(f, fpage, stage, true, false);   // all lanes have their scores (the vote): K has been read
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -675,45 +743,72 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                 }
             }
         } else {
-            // p times the value's scale, as the sum of two bf16 (16 bits of it), times the exact
-            // int8: bf16 has the range that an f16 product of two small numbers lacks
-            const int key = (lane & 7) + (lane >> 4) * 8;
-            const int swz = HD == 128 ? (key & 7) : ((key >> 1) & 3);
+            // The weights p times scale of this unit's 32 keys as 16-bit integers (two bytes, two
+            // products) per head and block, relative to the largest p times the largest scale:
+            // each is off by 2^-17 of that at most.
+            const int swz = HD == 128 ? (lane & 7) : ((lane >> 1) & 3);
+            float sv[4][NB], rv[NB], vmax[NB];
+            scales_of(vsc, sv);
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int k = 0; k < NB; ++k) {
+                float v = fmaxf(fmaxf(fabsf(sv[0][k]), fabsf(sv[1][k])), fmaxf(fabsf(sv[2][k]), fabsf(sv[3][k])));
 #pragma unroll
-                for (int k = 0; k < NB; ++k) {
-                    const float s0 = __half2float(vsc[scale_at(a * 16 + r8) + k]);
-                    const float s1 = __half2float(vsc[scale_at(a * 16 + r8 + 8) + k]);
-                    uint32_t hi[NT][2], lo[NT][2];
+                for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(NCM_FULL, v, x));
+                vmax[k] = fmaxf(v, 0x1p-24f);
+                rv[k] = __fdividef(65534.0f, vmax[k]);
+            }
+            float pmax[NT][2];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float v = fmaxf(fmaxf(s[0][t][j], s[0][t][j + 2]), fmaxf(s[1][t][j], s[1][t][j + 2]));
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(NCM_FULL, v, x));
+                    v = fmaxf(v, 0x1p-60f);
+                    const float r = __fdividef(1.0f, v);
+                    pmax[t][j] = v * (1.0f / 65534.0f);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) { s[a][t][j] *= r; s[a][t][j + 2] *= r; }
+                }
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        uint32_t w[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float x0 = s[a][t][2 * j] * (j ? s1 : s0), x1 = s[a][t][2 * j + 1] * (j ? s1 : s0);
-                            const uint32_t h = pack2(true, x0, x1);
-                            hi[t][j] = transposed(h);
-                            lo[t][j] = transposed(pack2(true, x0 - __uint_as_float(h << 16),
-                                                        x1 - __uint_as_float(h & 0xffff0000u)));
+                            const float f = sv[2 * a + j][k] * rv[k];
+                            w[j] = transposed(__byte_perm(__float_as_uint(fmaf(s[a][t][2 * j], f, 0x1p23f)),
+                                                          __float_as_uint(fmaf(s[a][t][2 * j + 1], f, 0x1p23f)), 0x5410));
                         }
-                    const int col = 2 * k + ((lane >> 3) & 1);
+                        hi[t][a] = __byte_perm(w[0], w[1], 0x7531);   // keys 16 a + 2 c4, + 1, + 8, + 9
+                        lo[t][a] = __byte_perm(w[0], w[1], 0x6420);
+                    }
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {   // 16 values of d; x[i]: keys 8 i + 2 c4, + 1, of d 2 r8 and 2 r8 + 1
                     uint32_t x[4];
-                    ldsm4t(x, va + (a * 16 + key) * HD + ((col ^ swz) << 4));
+                    ldsm4t(x, va + lane * HD + (((2 * k + g) ^ swz) << 4));
+                    const uint32_t a0 = __byte_perm(x[0], x[1], 0x6420), a1 = __byte_perm(x[0], x[1], 0x7531);
+                    const uint32_t a2 = __byte_perm(x[2], x[3], 0x6420), a3 = __byte_perm(x[2], x[3], 0x7531);
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {   // x[g]: keys 0-7, x[g + 2]: keys 8-15 of 16 values of d
-                        const uint32_t a0 = int8_pair<true>(x[g]), a1 = int8_pair<true>(x[g] >> 8);
-                        const uint32_t a2 = int8_pair<true>(x[g + 2]), a3 = int8_pair<true>(x[g + 2] >> 8);
+                    for (int t = 0; t < NT; ++t) {
+                        float h[4], w[4];
+                        imma16832<true>(h, a0, a1, a2, a3, hi[t][0], hi[t][1]);
+                        imma16832<true>(w, a0, a1, a2, a3, lo[t][0], lo[t][1]);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            mma16816<true>(o[2 * k + g][t], a0, a1, a2, a3, hi[t][0], hi[t][1]);
-                            mma16816<true>(o[2 * k + g][t], a0, a1, a2, a3, lo[t][0], lo[t][1]);
-                        }
+                        for (int j = 0; j < 4; ++j)
+                            o[2 * k + g][t][j] = fmaf(joined(h[j], w[j]), pmax[t][j & 1] * vmax[k], o[2 * k + g][t][j]);
                     }
                 }
+            }
         }
         __syncwarp();
         if (fetched < count) {
-            issue(f, fpage, stage);
+            issue(f, fpage, stage, !ONE, true);
             next(f);
             if (++fetched < count) fpage = page_at(f, lane);
         }
@@ -723,7 +818,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             const bool whole = c.u + 1 == c.n && i - began + 1 == c.n;
             sum_lanes();
             if (whole) {
-                const int h = c.hk / p.nchunk, ch = c.hk % p.nchunk;
+                const int h = head_of(c.hk), ch = c.hk - h * p.nchunk;
                 const int heads = min(p.chunk, p.group - ch * p.chunk);
                 uint16_t* out = static_cast<uint16_t*>(p.out) + c.b * p.out_stride +
                                 (int64_t)(h * p.group + ch * p.chunk) * HD;
@@ -769,7 +864,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     for (int e = 0; e < 2 * W;) {
         const int4 seg = *reinterpret_cast<const int4*>(ent + 4 * e);
         if (seg.x < 0) { ++e; continue; }
-        const int b = seg.x, hk = seg.y, sb = seg.z, se = seg.w, h = hk / p.nchunk, ch = hk - h * p.nchunk;
+        const int b = seg.x, hk = seg.y, sb = seg.z, se = seg.w, h = head_of(hk), ch = hk - h * p.nchunk;
         uint32_t of = 0;   // the entries of this segment: those up to the next one's first
         int e1 = e;
         for (; e1 < 2 * W; ++e1) {
@@ -962,7 +1057,7 @@ int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
     const int stage = 2 * (kUnit * HD * (Q8 ? 1 : 2) + (Q8 ? 512 : 0));
     const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (2 * W + 2) * 4 + (2 * p.batch + 1) * 4;
     int n = 1;   // stages: as many as fit, 8 at most
-    while (n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
+    while (!one_stage(HD, NT) && n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
     p.nstages = n;
     auto fn = paged_attn_kernel<BF16, Q8, HD, NT, W>;
     if (int r = set_smem_limit((const void*)fn, kPagedSmem)) return r;
@@ -972,9 +1067,14 @@ int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
 template <bool BF16, bool Q8>
 int paged_attn_pick(PagedAttnParams& p, int hd, int grid, cudaStream_t s) {
     const bool two = p.chunk > 8;
-    if (hd == 64) return two ? paged_attn_run<BF16, Q8, 64, 2, W64>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1, W64>(p, grid, s);
-    if (two) return paged_attn_run<BF16, Q8, 128, 2, Q8 ? WQ2 : 4>(p, grid, s);
-    return paged_attn_run<BF16, Q8, 128, 1, Q8 ? WQ1 : W128>(p, grid, s);
+    // Warps of a CTA.  Q8_0 is bound by instructions and takes as many as its registers allow (48
+    // sequences of 300 to 6000, 32 / 8 heads of 128: 8 warps 79.9 us, 12 77.5); 16-bit values
+    // need only enough in flight (64 sequences of 1 to 8192, heads of 128: 6 warps of two stages
+    // 177 us, 7 of one 168, 8 171, 9 175; heads of 64: 8 warps 87.1 us, 12 88.9).
+    if (hd == 64)
+        return two ? paged_attn_run<BF16, Q8, 64, 2, 8>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1, Q8 ? 12 : 8>(p, grid, s);
+    if (two) return paged_attn_run<BF16, Q8, 128, 2, Q8 ? 8 : 4>(p, grid, s);
+    return paged_attn_run<BF16, Q8, 128, 1, Q8 ? 12 : 7>(p, grid, s);
 }
 
 int bad(const char* what) { return set_error(NCM_EINVAL, what); }
@@ -1086,7 +1186,7 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     p.part = (float*)((char*)workspace + 4096);
     p.err = err;
     // positions in the row of units, padded to pieces, fit 32 bits
-    const int64_t most = ((int64_t)table_width * kv->page_size / (kUnit * kPiece * 8) + 1) * kPiece * 8 * kv->kv_heads * p.nchunk;
+    const int64_t most = ((int64_t)table_width * kv->page_size / (kUnit * kPiece * 4) + 1) * kPiece * 12 * kv->kv_heads * p.nchunk;
     const int step = (int)std::min<int64_t>(kPagedBatch, (int64_t)0x7fff0000 / most);
     if (step < 1) return set_error(NCM_EUNSUPPORTED, "a sequence's pages hold too many tokens for so many heads");
     cudaStream_t s = (cudaStream_t)stream;

@@ -7,7 +7,11 @@ An attention output o = sum w_j v_j carries its own rounding (u |o|), the roundi
 p_j to 16 bits (u sum w_j |v_j|), the f32 error of the scores, which moves each p_j by at
 most e = 2^-24 (head_dim + 4) * max |q||k| scale + 2^-21 relative (and the sum as much), the f32
 sums over n keys (n 2^-24) and, for f16, the 2^-25 that a p below 2^-14 may be off, the
-largest p being at least one."""
+largest p being at least one.  Over Q8_0 the products are of integers: a query value is a
+multiple of amax / 32512 of its block of 32, so off by amax / 65024, which moves a score by
+scale * sum |k_d| amax / 65024 at most (e grows by twice that); and p times a value's scale is
+a multiple of 1 / 65534 of the largest p times the largest scale among 32 keys (from a multiple
+of 32 on), so each of the 32 adds at most 127 / 131068 of that product to the error."""
 import numpy as np
 import pytest
 import torch
@@ -74,11 +78,14 @@ class Cache:
         pos = torch.arange(n, device="cuda")
         pg, off = self.table[i].long()[pos // self.page], pos % self.page
         y = x[pg, :, off].double()
+        if which == "v_scales":
+            return s[pg, :, off] if s is not None else None
         return y * s[pg, :, off].double().repeat_interleave(32, -1) if self.kind == "q8_0" else y
 
 
-def attend64(q, k, v, scale, qkind, hd):
-    """One query [heads, hd] over [n, kvh, hd] in 64 bits: the output and its tolerance."""
+def attend64(q, k, v, scale, qkind, hd, v_scales=None):
+    """One query [heads, hd] over [n, kvh, hd] in 64 bits: the output and its tolerance.
+    v_scales [n, kvh, hd / 32]: of a Q8_0 cache."""
     heads, g = q.shape[0], q.shape[0] // k.shape[1]
     if k.shape[0] == 0:
         return torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
@@ -90,6 +97,14 @@ def attend64(q, k, v, scale, qkind, hd):
     n, u = k.shape[0], U[qkind]
     e = 2 * (2.0 ** -24 * (hd + 4) * top + 2.0 ** -21) + n * 2.0 ** -24
     small = 2.0 ** -25 * (1 + n * v.abs().amax()) if qkind == "f16" else 0.0
+    if v_scales is not None:
+        step = q.double().abs().unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1) / 65024
+        e = e + 2 * (torch.einsum("hd,nhd->hn", step, k.abs()) * scale).amax(-1)[:, None]
+        pad = -n % 32
+        wu = torch.nn.functional.pad(w, (0, pad)).unflatten(-1, (-1, 32)).amax(-1)                               # [h, units]
+        su = torch.nn.functional.pad(v_scales.double(), (0, 0, 0, 0, 0, pad)).unflatten(0, (-1, 32)).amax(1)    # [units, kvh, hd / 32]
+        su = su.repeat_interleave(g, 1).repeat_interleave(32, -1)
+        small = small + torch.einsum("hu,uhd->hd", wu, su) * (32 * 127 / 131068)
     return o, u * o.abs() + (u + e) * a * (1 + u) + small
 
 
@@ -105,7 +120,7 @@ def attend(ncm, c, q, lengths, heads, qkind, out=None, scale=0.0, err=None, spac
 def check(c, q, out, lengths, qkind, scale=None):
     scale = c.hd ** -0.5 if scale is None else scale
     for i, n in enumerate(lengths):
-        ref, tol = attend64(q[i], c.rows("k", i, max(n, 0)), c.rows("v", i, max(n, 0)), scale, qkind, c.hd)
+        ref, tol = attend64(q[i], c.rows("k", i, max(n, 0)), c.rows("v", i, max(n, 0)), scale, qkind, c.hd, c.rows("v_scales", i, max(n, 0)))
         off = (out[i].double() - ref).abs()
         assert bool((off <= tol).all()), (i, n, float((off - tol).max()), float(off.max()))
 
