@@ -1111,7 +1111,8 @@ extern "C" ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, cons
             return bad("q, k and v rows must be 16-byte aligned and at least a token apart");
     }
     if (!aligned16(q_out)) return bad("q_out must be 16-byte aligned");
-    const void* check[] = {k, v, kv->k, kv->v, kv->k_scales, kv->v_scales, lengths, page_table, rope, src[0], q_out};
+    const void* check[] = {k, v, kv->k, kv->v, kv->k_scales, kv->v_scales, lengths, page_table, cu_tokens, rope, src[0],
+                           heads ? q_out : nullptr, err};
     for (const void* c : check)
         if (c)
             if (const char* e = device_pointer_error(c)) return bad(e);
@@ -1167,7 +1168,7 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     size_t need = 0;
     if (ncm_paged_attention_workspace(heads, kv->kv_heads, hd, &need) || workspace_bytes < need)
         return bad("workspace smaller than ncm_paged_attention_workspace says");
-    const void* check[] = {out, q, kv->k, kv->v, kv->k_scales, kv->v_scales, lengths, page_table, workspace};
+    const void* check[] = {out, q, kv->k, kv->v, kv->k_scales, kv->v_scales, lengths, page_table, workspace, err};
     for (const void* c : check)
         if (c)
             if (const char* e = device_pointer_error(c)) return bad(e);

@@ -226,6 +226,7 @@ __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix
     t.q0 = min(max(q.x, 0), p.total_q); t.nq = min(max(q.y, t.q0), p.total_q) - t.q0;
     t.k0 = min(max(k.x, 0), p.total_k); t.nk = min(max(k.y, t.k0), p.total_k) - t.k0;
     t.t0 = (block - prefix[lo]) * 2 * p.tokens;
+    if (t.t0 < 0) t.t0 = t.nq;   // sums that ran over, from cu_q entries out of order: an item without rows
     t.shift = t.nk - t.nq;
     int least = t.nk;                                             // keys that every row sees
 #pragma unroll
@@ -733,9 +734,10 @@ extern "C" ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const 
             return bad("rows must be 16-byte aligned and at least a token apart");
     }
     if (total_k == 0) { k = q; v = q; k_stride = q_stride; v_stride = q_stride; }   // never read: no row sees a key
-    const void* check[] = {out, q, k, v, cu_q, cu_k};
+    const void* check[] = {out, q, k, v, cu_q, cu_k, err};
     for (const void* c : check)
-        if (const char* e = device_pointer_error(c)) return bad(e);
+        if (c)
+            if (const char* e = device_pointer_error(c)) return bad(e);
     if (!encode_tiled_fn()) return set_error(NCM_ECUDA, "cuTensorMapEncodeTiled not available");
     PromptParams p;
     memset(&p, 0, sizeof p);
