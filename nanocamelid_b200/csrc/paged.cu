@@ -617,7 +617,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                 }
             }
         };
-        if (!mbar_wait(bar + 2 * stage, phase, kPagedWaitNs)) { failed = true; break; }
+        // (the vote brings the lanes together again: ldmatrix and mma want them all)
+        if (!__all_sync(NCM_FULL, mbar_wait(bar + 2 * stage, phase, kPagedWaitNs))) { failed = true; break; }
         // scores: rows = keys, columns = heads
         float s[2][NT][4];
 #pragma unroll
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     l[t][j & 1] += s[a][t][j];
                 }
             }
-        if (!mbar_wait(bar + 2 * stage + 1, phase, kPagedWaitNs)) { failed = true; break; }
+        if (!__all_sync(NCM_FULL, mbar_wait(bar + 2 * stage + 1, phase, kPagedWaitNs))) { failed = true; break; }
         if (valid < kUnit) {   // rows behind the last key may hold anything: zero x NaN is NaN
             constexpr int ROW = Q8 ? HD : 128;
             for (int e = lane; e < (kUnit - valid) * (ROW / 16); e += 32) {
