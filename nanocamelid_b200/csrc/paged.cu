@@ -883,13 +883,13 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         for (int x = tid; x < heads * (HD / 4); x += W * 32) {
             const int head = x / (HD / 4), d = 4 * (x % (HD / 4));
             float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int y = 0; y < 2 * W; ++y)
-                if (of >> y & 1) top = fmaxf(top, ((y & 1) ? last_ml : first_ml)[((y >> 1) * GH + head) * 2]);
+            for (uint32_t left = of; left; left &= left - 1) {
+                const int y = __ffs(left) - 1;
+                top = fmaxf(top, ((y & 1) ? last_ml : first_ml)[((y >> 1) * GH + head) * 2]);
+            }
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int y = 0; y < 2 * W; ++y) {
-                if (!(of >> y & 1)) continue;
+            for (uint32_t left = of; left; left &= left - 1) {
+                const int y = __ffs(left) - 1;
                 const float* ml = ((y & 1) ? last_ml : first_ml) + ((y >> 1) * GH + head) * 2;
                 const float4 v = *reinterpret_cast<const float4*>(((y & 1) ? last : first) + ((y >> 1) * GH + head) * HD + d);
                 const float w = part_weight(ml[0], top);

@@ -37,10 +37,9 @@ constexpr int kRows = 128;               // query rows of a tile, and keys of a 
 constexpr int kUnitKeys = 64;            // keys of one step of the softmax
 constexpr int kPromptThreads = 384;
 constexpr int kPromptBatch = 1024;       // sequences of one launch
-#ifndef POLY8
-#define POLY8 2
-#endif
-constexpr int kPolyOf8 = POLY8;
+// Exponentials of every eight that the FMA pipe computes: 0, 1, 2, 3 take 107.5, 104.5, 102.1,
+// 103.5 us (12 ragged prompts, 32 / 8 heads of 64) and 146, 144, 143.5, 146 (4 chunks, 64 / 8 of 128).
+constexpr int kPolyOf8 = 2;
 constexpr int kPromptSmem = 232448;
 constexpr uint64_t kPromptWaitNs = 2000000000ull;
 
@@ -449,12 +448,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 if (t.n1 > 0) scores(1, 0);
                 give_back(empty + slot_of(0));
                 if (n == 1) give_back(q_empty);
+                // V of tile j and K of tile j + 1 are waited for a step ahead, while the products of
+                // query tile 0 run: the ring holds both beside the two in use.
+                static_assert(NST >= 4, "the ring holds two tiles of K and of V");
+                if (!arrived(1) || (n > 1 && !arrived(2))) break;
                 for (int j = 0; j < n && ok; ++j) {
-                    if (!arrived(2 * j + 1)) break;
-                    if (j + 1 < n && !arrived(2 * j + 2)) break;
                     const uint32_t v = ring + slot_of(2 * j + 1) * L::kTile;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
+                    for (int x = 0; x < 2; ++x) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int u = 2 * j + h;
@@ -472,6 +473,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                             __syncwarp();
                             if (h == 1 && u + 1 < t.n(x)) scores(x, 2 * j + 2);
                         }
+                        if (x == 0) {
+                            if (j + 1 < n) arrived(2 * j + 3);
+                            if (j + 2 < n) arrived(2 * j + 4);
+                        }
+                    }
                     if (elected()) {
                         mma_commit(empty + slot_of(2 * j + 1));
                         if (j + 1 < n) mma_commit(empty + slot_of(2 * j + 2));
