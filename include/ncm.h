@@ -137,7 +137,7 @@ typedef struct {
                             0: kv_heads * page_size * head_dim.  Lets K and V share pages. */
     void* k;            /* [pages][kv_heads][page_size][head_dim] 16-bit values, or int8 for Q8_0 */
     void* v;
-    void* k_scales;     /* Q8_0: f16 [pages][kv_heads][page_size][head_dim / 32], else NULL */
+    void* k_scales;     /* Q8_0: f16 [pages][kv_heads][page_size][head_dim / 32], not negative; else NULL */
     void* v_scales;
 } ncm_paged_kv;
 
@@ -155,8 +155,8 @@ typedef struct {
  * NCM_ROPE_PAIRS rotates (2i, 2i+1) for i < rope_half (inference.rs:904-933), the rest passes
  * unchanged; NCM_ROPE_HALVES rotates (i, i + head_dim/2), rope_half = head_dim/2.
  * Q8_0: per 32 values scale = max|x| * (1 / 127) in f32, kept as f16 rounded toward zero, int8 =
- * round-half-away(x * (1 / scale)): ncm_model_set_kv_cache's rule but for its division.  A row whose position or page is out of
- * range is not written at all (NCM_DEVICE_BAD_ARG). */
+ * round-half-away(x * (1 / scale)): ncm_model_set_kv_cache's rule but for its division.
+ * A row whose position or page is out of range is not written at all (NCM_DEVICE_BAD_ARG). */
 #define NCM_ROPE_PAIRS 0
 #define NCM_ROPE_HALVES 1
 ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, const void* q, int64_t q_stride, const void* k,
@@ -174,11 +174,14 @@ ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, const void* q, 
  * Several rows of one sequence (a speculative batch) are passed as sequences of their own
  * that share a page table row's contents.  table_width * page_size <= 2^22; a longer length
  * is cut there and a page id out of range reads as zeros (both NCM_DEVICE_BAD_ARG).
- * scale 0 means 1 / sqrt(head_dim).  Softmax and sums are f32; the result does not depend on
- * the order in which the parts of a long sequence finish.
+ * scale 0 means 1 / sqrt(head_dim).  Softmax and sums are f32; p is rounded to q_type.  Over
+ * Q8_0 a query is taken as a multiple of its block's largest value / 32512 and p times the
+ * value's scale as a multiple of the largest such product among 32 keys / 65534.  The result
+ * does not depend on the order in which the parts of a long sequence finish.
  * workspace: at least ncm_paged_attention_workspace bytes, zeroed once before its first use
- * (each call leaves its counters zero again); calls that can overlap on the GPU need one
- * each, calls in stream order, graph replays among them, can share one. */
+ * (each call leaves its counters zero again, unless it ends with NCM_DEVICE_TIMEOUT); calls
+ * that can overlap on the GPU need one each, calls in stream order, graph replays among
+ * them, can share one. */
 ncm_status ncm_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t* bytes);
 ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_stride, const void* q, int64_t q_stride,
                                int q_type, int batch, int heads, const int* lengths, const int* page_table,
