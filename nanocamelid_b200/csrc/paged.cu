@@ -228,7 +228,9 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ attention of one token
 constexpr int kUnit = 32;              // keys that a warp takes at a time
-constexpr int kPiece = 8;              // units per warp up to which a segment stays in one CTA
+// Units per warp, once or twice as many, up to which a segment stays in one CTA.  2, 3, 4, 8: one
+// sequence of 4000 keys (32 / 8 heads of 128) 12.4, 13.4, 14.7, 20.3 us; of 500 keys 10.6, 9.8, 9.7, 9.8.
+constexpr int kPiece = 2;
 constexpr int kPagedBatch = 1024;      // sequences of one launch (their lengths lie in shared memory)
 constexpr int kPagedSmem = 232448;     // 227 KB
 
@@ -317,7 +319,7 @@ template <bool BF16> __device__ __forceinline__ float2 widen2(uint32_t w) {
 // A segment is one (sequence, key-value head, chunk of its query heads); its keys are cut in
 // units of 32.  All units of all segments lie in one row that is shared out evenly, first
 // over the CTAs, then over a CTA's warps; when there are so few that every CTA can take at
-// most `kPiece` units per warp of a single segment, the row is padded so that no CTA has
+// most `kPiece` units per warp (or twice that) of a single segment, the row is padded so that no CTA has
 // two segments: a segment that fits one CTA is then joined in shared memory alone (a join
 // over CTAs costs about 4 us).  Positions fit 32 bits: the host sees to it.  A place in the row:
 struct Place {
@@ -359,18 +361,18 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     float* first_ml = first + W * GH * HD;
     uint64_t* bars = reinterpret_cast<uint64_t*>(first_ml + W * GH * 2);   // [warp][stage][2]
     int* ent = reinterpret_cast<int*>(bars + W * nst * 2);       // [2 W][4]: sequence (-1: none), segment, begin, end
-    int* sums = ent + 2 * W * 4;                                 // [2 W + 2]
-    int* prefix = sums + 2 * W + 2;                                      // [batch + 1]
+    int* sums = ent + 2 * W * 4;                                 // [3 W + 1]
+    int* prefix = sums + 3 * W + 1;                                      // [batch + 1]
     int* lens = prefix + p.batch + 1;                            // [batch]
 
     // ---- lengths and their running sum of units, as they are and padded to pieces
     const int HK = p.kv_heads * p.nchunk;
-    constexpr int PIECE = kPiece * W;
-    bool pieces;
+    int piece = kPiece * W;   // 0: no padding
     {
         const int per = (p.batch + W * 32 - 1) / (W * 32);
         const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-        int sum = 0, sum_p = 0;
+        int sum = 0, sum_p = 0, sum_2p = 0;
+        auto pieces_of = [&](int n, int size) { return ((n + kUnit - 1) / kUnit + size - 1) / size; };
         const int cap = p.table_width << p.log2ps;
         for (int b = b0; b < b1; ++b) {
             int n = __ldg(p.lengths + b);
@@ -381,15 +383,17 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             n = max(n, 0);
             lens[b] = n;
             sum += (n + kUnit - 1) / kUnit;
-            sum_p += (n + kUnit * PIECE - 1) / (kUnit * PIECE);
+            sum_p += pieces_of(n, kPiece * W);
+            sum_2p += pieces_of(n, 2 * kPiece * W);
         }
-        int run = sum, run_p = sum_p;
+        int run = sum, run_p = sum_p, run_2p = sum_2p;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(NCM_FULL, run, o), v_p = __shfl_up_sync(NCM_FULL, run_p, o);
-            if (lane >= o) { run += v; run_p += v_p; }
+            const int v_2p = __shfl_up_sync(NCM_FULL, run_2p, o);
+            if (lane >= o) { run += v; run_p += v_p; run_2p += v_2p; }
         }
-        if (lane == 31) { sums[2 * warp] = run; sums[2 * warp + 1] = run_p; }
+        if (lane == 31) { sums[3 * warp] = run; sums[3 * warp + 1] = run_p; sums[3 * warp + 2] = run_2p; }
         if (tid < 2 * W) ent[4 * tid] = -1;
         if (lane == 0)
             for (int i = 0; i < 2 * nst; ++i) mbar_init(bars + warp * nst * 2 + i, 1);
@@ -397,19 +401,25 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         __syncthreads();
         run -= sum;
         run_p -= sum_p;
-        int all_p = 0;
+        run_2p -= sum_2p;
+        int all_p = 0, all_2p = 0;
         for (int w = 0; w < W; ++w) {
-            if (w < warp) { run += sums[2 * w]; run_p += sums[2 * w + 1]; }
-            all_p += sums[2 * w + 1];
+            if (w < warp) { run += sums[3 * w]; run_p += sums[3 * w + 1]; run_2p += sums[3 * w + 2]; }
+            all_p += sums[3 * w + 1];
+            all_2p += sums[3 * w + 2];
         }
-        pieces = all_p <= (int)gridDim.x / HK;
+        const int room = (int)gridDim.x / HK;
+        if (all_p > room) {
+            piece = all_2p > room ? 0 : 2 * kPiece * W;
+            run_p = run_2p;
+        }
         if (tid == 0) prefix[0] = 0;
         for (int b = b0; b < b1; ++b) {
-            if (pieces) {
-                run_p += (lens[b] + kUnit * PIECE - 1) / (kUnit * PIECE);
-                prefix[b + 1] = run_p * PIECE;
+            if (piece) {
+                run_p += pieces_of(lens[b], piece);
+                prefix[b + 1] = run_p * piece;
             } else {
-                run += (lens[b] + kUnit - 1) / kUnit;
+                run += pieces_of(lens[b], 1);
                 prefix[b + 1] = run;
             }
         }
@@ -422,7 +432,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                 store_out<BF16>(p.out, b * p.out_stride + i, make_float4(0.f, 0.f, 0.f, 0.f));
 
     const int total = prefix[p.batch] * HK;
-    const int share = pieces ? PIECE : max(PIECE, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int share = piece ? piece : max(W, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     const int u0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
     if (u0 >= total) return;
     Place c;
@@ -439,12 +449,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         c.u = rest - c.hk * stride;
     };
     find(u0);
-    const int u1 = pieces ? u0 + min(share, c.n - c.u) : (int)min((int64_t)total, (int64_t)u0 + share);
+    const int u1 = piece ? u0 + min(share, c.n - c.u) : (int)min((int64_t)total, (int64_t)u0 + share);
     const int per_warp = (u1 - u0 + W - 1) / W;
     const int w0 = min(u1, u0 + warp * per_warp), w1 = min(u1, w0 + per_warp);
     const int count = w1 - w0;
     if (count > 0) {
-        if (pieces) c.u += w0 - u0; else find(w0);
+        if (piece) c.u += w0 - u0; else find(w0);
     }
 
     // ---- this warp's units
@@ -926,11 +936,11 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                sums[2 * W] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
-                if (sums[2 * W]) p.counters[i0] = 0;
+                sums[3 * W] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
+                if (sums[3 * W]) p.counters[i0] = 0;
             }
             __syncthreads();
-            if (sums[2 * W]) {
+            if (sums[3 * W]) {
                 __threadfence();
                 const int np = i1 - i0 + 1;
                 auto part_of = [&](int i) { return (int64_t)(2 * (i0 + i) + (i == 0 ? 1 : 0)); };
@@ -1067,7 +1077,7 @@ int paged_maps(const ncm_paged_kv* kv, int box, PagedAttnParams& p) {
 template <bool BF16, bool Q8, int HD, int NT, int W>
 int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
     const int stage = 2 * (kUnit * HD * (Q8 ? 1 : 2) + (Q8 ? 512 : 0));
-    const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (2 * W + 2) * 4 + (2 * p.batch + 1) * 4;
+    const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (3 * W + 1) * 4 + (2 * p.batch + 1) * 4;
     int n = 1;   // stages: as many as fit, 8 at most
     while (!one_stage(HD, NT) && n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
     p.nstages = n;
@@ -1202,7 +1212,7 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     p.part = (float*)((char*)workspace + 4096);
     p.err = err;
     // positions in the row of units, padded to pieces, fit 32 bits
-    const int64_t most = ((int64_t)table_width * kv->page_size / (kUnit * kPiece * 4) + 1) * kPiece * 12 * kv->kv_heads * p.nchunk;
+    const int64_t most = ((int64_t)table_width * kv->page_size / (kUnit * kPiece * 4) + 1) * kPiece * 24 * kv->kv_heads * p.nchunk;
     const int step = (int)std::min<int64_t>(kPagedBatch, (int64_t)0x7fff0000 / most);
     if (step < 1) return set_error(NCM_EUNSUPPORTED, "a sequence's pages hold too many tokens for so many heads");
     cudaStream_t s = (cudaStream_t)stream;

@@ -104,11 +104,19 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define NCM_R8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
 #define NCM_W8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+#define NCM_U8(r, i) "+r"((r)[i]), "+r"((r)[i + 1]), "+r"((r)[i + 2]), "+r"((r)[i + 3]), "+r"((r)[i + 4]), "+r"((r)[i + 5]), "+r"((r)[i + 6]), "+r"((r)[i + 7])
+// Waits for this thread's TMEM loads.  It names what they loaded, so that no use of it is moved
+// before the wait (`landed` does that for further registers).
+__device__ __forceinline__ void wait_ld(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : NCM_U8(r, 0), NCM_U8(r, 8), NCM_U8(r, 16), NCM_U8(r, 24)::"memory");
+}
+__device__ __forceinline__ void landed(uint32_t* r) {
+    asm volatile("" : NCM_U8(r, 0), NCM_U8(r, 8), NCM_U8(r, 16), NCM_U8(r, 24)::"memory");
+}
 // 32 columns of this warp's 32 lanes (one row per lane).
 __device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
     asm volatile(
@@ -553,7 +561,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 uint32_t s[64];
                 tmem_ld32(s, s_unit);
                 tmem_ld32(s + 32, s_unit + 32);
-                wait_ld();
+                wait_ld(s);
+                landed(s + 32);
                 const bool masked = (u + 1) * kUnitKeys > t.seen;
                 if (masked) {
                     const int left = limit - u * kUnitKeys;             // columns up to this one are seen
@@ -583,7 +592,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                         for (int c = 0; c < HD; c += 32) {
                             uint32_t o[32];
                             tmem_ld32(o, o_at + c);
-                            wait_ld();
+                            wait_ld(o);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
                             tmem_st32(o_at + c, o);
@@ -643,7 +652,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 uint32_t o[32];
                 if (units > 0) {
                     tmem_ld32(o, o_at + c);
-                    wait_ld();
+                    wait_ld(o);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
