@@ -901,32 +901,35 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         const int slot = sb < u0 ? 0 : 1;
         float* rows = p.part + (int64_t)(2 * blockIdx.x + slot) * p.chunk * HD;
         float* mls = p.part + (int64_t)2 * gridDim.x * p.chunk * HD;
-        for (int x = tid; x < heads * (HD / 4); x += W * 32) {
-            const int head = x / (HD / 4), d = 4 * (x % (HD / 4));
-            float top = -INFINITY, sum = 0.0f;
-            for (uint32_t left = of; left; left &= left - 1) {
-                const int y = __ffs(left) - 1;
-                top = fmaxf(top, ((y & 1) ? last_ml : first_ml)[((y >> 1) * GH + head) * 2]);
-            }
+        static_assert(2 * W <= 32, "an entry per lane");
+        for (int head = warp; head < heads; head += W) {   // lane y: entry y; then lane: four values of d
+            const bool has = lane < 2 * W && (of >> lane & 1);
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (has) ml = *reinterpret_cast<const float2*>(((lane & 1) ? last_ml : first_ml) + ((lane >> 1) * GH + head) * 2);
+            float top = ml.x;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(NCM_FULL, top, x));
+            const float weight = part_weight(ml.x, top);
+            float sum = weight * ml.y;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(NCM_FULL, sum, x);
+            const int d = 4 * lane;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             for (uint32_t left = of; left; left &= left - 1) {
                 const int y = __ffs(left) - 1;
-                const float* ml = ((y & 1) ? last_ml : first_ml) + ((y >> 1) * GH + head) * 2;
+                const float w = __shfl_sync(NCM_FULL, weight, y);
+                if (d >= HD) continue;
                 const float4 v = *reinterpret_cast<const float4*>(((y & 1) ? last : first) + ((y >> 1) * GH + head) * HD + d);
-                const float w = part_weight(ml[0], top);
                 acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
                 acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
-                sum = fmaf(w, ml[1], sum);
             }
+            if (d >= HD) continue;
             if (inside) {
                 const float inv = 1.0f / sum;
                 store_out<BF16>(p.out, out_at + head * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
             } else {
                 *reinterpret_cast<float4*>(rows + head * HD + d) = acc;
-                if (d == 0) {
-                    float* ml = mls + ((int64_t)(2 * blockIdx.x + slot) * p.chunk + head) * 2;
-                    ml[0] = top; ml[1] = sum;
-                }
+                if (d == 0) *reinterpret_cast<float2*>(mls + ((int64_t)(2 * blockIdx.x + slot) * p.chunk + head) * 2) = make_float2(top, sum);
             }
         }
         if (!inside) {
