@@ -13,11 +13,14 @@
 //   10, 11    look over the V tiles at the mask's edge: a key that a mask hides has p = 0, but
 //             0 x infinity is not 0, so what is not finite there is taken out and given back
 //             in the epilogue to the rows that do see it.
-// While one tile's softmax runs, the tensor cores work on the other's products.  (A warp of its
-// own for each tile's products was slower, 579 us against 523 at one prompt of 8192, 32 / 8
-// heads of 128; scores in units of 64 keys, double buffered, too: 560 us, since a product
-// with N = 64 takes as long as one with N = 128.)  The softmax takes a tile's 128 keys in two steps of 64, whose p the tensor cores take one by
-// one.  TMEM columns: 128 x: S of tile x, and over it P, 64 h the step's; 256 + 128 x: O.
+// While one tile's softmax runs, the tensor cores work on the other's products.  The softmax
+// takes a tile's 128 keys in two steps of 64, whose p the tensor cores take one by one.
+// TMEM columns: 128 x: S of tile x, and over it P, 64 h the step's; 256 + 128 x: O.
+// What was slower, at one prompt of 8192 (32 / 8 heads of 128, 523 us then): an issuing warp for
+// each tile (579), sixteen softmax warps (530), scores in units of 64 keys, double buffered (560:
+// a product with N = 64 takes 50 cycles of the tensor cores, one with N = 128 64); and with heads
+// of 64, where TMEM has room for it, P beside S, so that the next scores need not wait for the
+// products (12 ragged prompts: 111 us against 102).
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
@@ -280,7 +283,7 @@ struct Layout {
     static constexpr int kBars = kRing + kStages * kTile;   // barriers, then a few words, then prefix
     static constexpr int kWords = kBars + 8 * (3 * kStages + 16);   // 16-byte aligned: NST is even
     static constexpr int kNext = kWords + 4 * 32;           // [2] answers of 16 bytes
-    static constexpr int kStore = (kNext + 32 + 127) / 128 * 128;   // 2 KB per softmax warp: 32 rows of 32 output values
+    static constexpr int kStore = (kNext + 32 + 127) / 128 * 128;   // 2 KB per softmax warp: 32 rows of 32 values
     static constexpr int kPrefix = kStore + 8 * 2048;       // running sums of blocks, cu_q, cu_k: batch + 1 each
 };
 
