@@ -228,9 +228,10 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ attention of one token
 constexpr int kUnit = 32;              // keys that a warp takes at a time
-// Units per warp, once or twice as many, up to which a segment stays in one CTA.  2, 3, 4, 8: one
-// sequence of 4000 keys (32 / 8 heads of 128) 12.4, 13.4, 14.7, 20.3 us; of 500 keys 10.6, 9.8, 9.7, 9.8.
-constexpr int kPiece = 2;
+// Units per warp up to which a segment stays in one CTA: 1, 2 or 4, the first with which there are
+// CTAs enough.  One sequence of 4000 keys (32 / 8 heads of 128) takes 11.5 us with 1 (and the join over
+// CTAs that it means), 12.0 with 2, 13.4 with 3, 14.7 with 4; one of 16000 20.9 with 2 and 4, 22.4 without.
+constexpr int kPieces = 3;
 constexpr int kPagedBatch = 1024;      // sequences of one launch (their lengths lie in shared memory)
 constexpr int kPagedSmem = 232448;     // 227 KB
 
@@ -319,7 +320,7 @@ template <bool BF16> __device__ __forceinline__ float2 widen2(uint32_t w) {
 // A segment is one (sequence, key-value head, chunk of its query heads); its keys are cut in
 // units of 32.  All units of all segments lie in one row that is shared out evenly, first
 // over the CTAs, then over a CTA's warps; when there are so few that every CTA can take at
-// most `kPiece` units per warp (or twice that) of a single segment, the row is padded so that no CTA has
+// most 4 units per warp of a single segment, the row is padded so that no CTA has
 // two segments: a segment that fits one CTA is then joined in shared memory alone (a join
 // over CTAs costs about 4 us).  Positions fit 32 bits: the host sees to it.  A place in the row:
 struct Place {
@@ -361,18 +362,20 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     float* first_ml = first + W * GH * HD;
     uint64_t* bars = reinterpret_cast<uint64_t*>(first_ml + W * GH * 2);   // [warp][stage][2]
     int* ent = reinterpret_cast<int*>(bars + W * nst * 2);       // [2 W][4]: sequence (-1: none), segment, begin, end
-    int* sums = ent + 2 * W * 4;                                 // [3 W + 1]
-    int* prefix = sums + 3 * W + 1;                                      // [batch + 1]
+    int* sums = ent + 2 * W * 4;                                 // [4 W + 1]
+    int* prefix = sums + 4 * W + 1;                                      // [batch + 1]
     int* lens = prefix + p.batch + 1;                            // [batch]
 
     // ---- lengths and their running sum of units, as they are and padded to pieces
     const int HK = p.kv_heads * p.nchunk;
-    int piece = kPiece * W;   // 0: no padding
+    int piece = 0;   // units of a piece; 0: no padding
     {
         const int per = (p.batch + W * 32 - 1) / (W * 32);
         const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-        int sum = 0, sum_p = 0, sum_2p = 0;
+        int sum[kPieces + 1], run[kPieces + 1];   // in units, and in pieces of W, 2 W, 4 W
         auto pieces_of = [&](int n, int size) { return ((n + kUnit - 1) / kUnit + size - 1) / size; };
+#pragma unroll
+        for (int i = 0; i <= kPieces; ++i) sum[i] = 0;
         const int cap = p.table_width << p.log2ps;
         for (int b = b0; b < b1; ++b) {
             int n = __ldg(p.lengths + b);
@@ -382,46 +385,39 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             }
             n = max(n, 0);
             lens[b] = n;
-            sum += (n + kUnit - 1) / kUnit;
-            sum_p += pieces_of(n, kPiece * W);
-            sum_2p += pieces_of(n, 2 * kPiece * W);
-        }
-        int run = sum, run_p = sum_p, run_2p = sum_2p;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(NCM_FULL, run, o), v_p = __shfl_up_sync(NCM_FULL, run_p, o);
-            const int v_2p = __shfl_up_sync(NCM_FULL, run_2p, o);
-            if (lane >= o) { run += v; run_p += v_p; run_2p += v_2p; }
+            for (int i = 0; i <= kPieces; ++i) sum[i] += pieces_of(n, i ? W << (i - 1) : 1);
         }
-        if (lane == 31) { sums[3 * warp] = run; sums[3 * warp + 1] = run_p; sums[3 * warp + 2] = run_2p; }
+#pragma unroll
+        for (int i = 0; i <= kPieces; ++i) {
+            run[i] = sum[i];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(NCM_FULL, run[i], o);
+                if (lane >= o) run[i] += v;
+            }
+        }
+        if (lane == 31) *reinterpret_cast<int4*>(sums + 4 * warp) = make_int4(run[0], run[1], run[2], run[3]);
         if (tid < 2 * W) ent[4 * tid] = -1;
         if (lane == 0)
             for (int i = 0; i < 2 * nst; ++i) mbar_init(bars + warp * nst * 2 + i, 1);
         fence_mbar_init();
         __syncthreads();
-        run -= sum;
-        run_p -= sum_p;
-        run_2p -= sum_2p;
-        int all_p = 0, all_2p = 0;
+        int4 before = make_int4(0, 0, 0, 0), all = before;
         for (int w = 0; w < W; ++w) {
-            if (w < warp) { run += sums[3 * w]; run_p += sums[3 * w + 1]; run_2p += sums[3 * w + 2]; }
-            all_p += sums[3 * w + 1];
-            all_2p += sums[3 * w + 2];
+            const int4 v = *reinterpret_cast<const int4*>(sums + 4 * w);
+            if (w < warp) { before.x += v.x; before.y += v.y; before.z += v.z; before.w += v.w; }
+            all.y += v.y; all.z += v.z; all.w += v.w;
         }
         const int room = (int)gridDim.x / HK;
-        if (all_p > room) {
-            piece = all_2p > room ? 0 : 2 * kPiece * W;
-            run_p = run_2p;
-        }
+        int at = before.x + run[0] - sum[0];
+        if (all.y <= room) { piece = W; at = before.y + run[1] - sum[1]; }
+        else if (all.z <= room) { piece = 2 * W; at = before.z + run[2] - sum[2]; }
+        else if (all.w <= room) { piece = 4 * W; at = before.w + run[3] - sum[3]; }
         if (tid == 0) prefix[0] = 0;
         for (int b = b0; b < b1; ++b) {
-            if (piece) {
-                run_p += pieces_of(lens[b], piece);
-                prefix[b + 1] = run_p * piece;
-            } else {
-                run += pieces_of(lens[b], 1);
-                prefix[b + 1] = run;
-            }
+            at += piece ? pieces_of(lens[b], piece) : pieces_of(lens[b], 1);
+            prefix[b + 1] = piece ? at * piece : at;
         }
         __syncthreads();
     }
@@ -939,11 +935,11 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                sums[3 * W] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
-                if (sums[3 * W]) p.counters[i0] = 0;
+                sums[4 * W] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
+                if (sums[4 * W]) p.counters[i0] = 0;
             }
             __syncthreads();
-            if (sums[3 * W]) {
+            if (sums[4 * W]) {
                 __threadfence();
                 const int np = i1 - i0 + 1;
                 auto part_of = [&](int i) { return (int64_t)(2 * (i0 + i) + (i == 0 ? 1 : 0)); };
@@ -1080,7 +1076,7 @@ int paged_maps(const ncm_paged_kv* kv, int box, PagedAttnParams& p) {
 template <bool BF16, bool Q8, int HD, int NT, int W>
 int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
     const int stage = 2 * (kUnit * HD * (Q8 ? 1 : 2) + (Q8 ? 512 : 0));
-    const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (3 * W + 1) * 4 + (2 * p.batch + 1) * 4;
+    const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (4 * W + 1) * 4 + (2 * p.batch + 1) * 4;
     int n = 1;   // stages: as many as fit, 8 at most
     while (!one_stage(HD, NT) && n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
     p.nstages = n;
@@ -1215,7 +1211,7 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     p.part = (float*)((char*)workspace + 4096);
     p.err = err;
     // positions in the row of units, padded to pieces, fit 32 bits
-    const int64_t most = ((int64_t)table_width * kv->page_size / (kUnit * kPiece * 4) + 1) * kPiece * 24 * kv->kv_heads * p.nchunk;
+    const int64_t most = ((int64_t)table_width * kv->page_size / kUnit + 1 + 48) * kv->kv_heads * p.nchunk;   // 4 * 12: a piece
     const int step = (int)std::min<int64_t>(kPagedBatch, (int64_t)0x7fff0000 / most);
     if (step < 1) return set_error(NCM_EUNSUPPORTED, "a sequence's pages hold too many tokens for so many heads");
     cudaStream_t s = (cudaStream_t)stream;
