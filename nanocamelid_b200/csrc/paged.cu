@@ -335,7 +335,7 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, float4 v) {
 }
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : ex2(m - top); }
 
-__host__ __device__ constexpr bool one_stage(int hd, int nt) { return hd == 128 && nt == 1; }
+__host__ __device__ constexpr bool one_stage(bool q8, int hd, int nt) { return nt == 1 && (hd == 128 || !q8); }
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(NCM_FULL, v, 0); }
 // One lane of a converged warp, in a form that the compiler knows for one.
 __device__ __forceinline__ bool elected() {
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     constexpr int SB = Q8 ? 512 : 0;                             // ... and of its scales
     constexpr int STAGE = 2 * (KB + SB);
     constexpr int KS = HD / 16, NB = HD / 32;
-    constexpr bool ONE = one_stage(HD, NT);                      // K and V of a unit are then fetched apart
+    constexpr bool ONE = one_stage(Q8, HD, NT);                      // K and V of a unit are then fetched apart
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c4 = lane & 3, r8 = lane >> 2;
     const int nst = p.nstages;
 
@@ -1078,7 +1078,7 @@ int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
     const int stage = 2 * (kUnit * HD * (Q8 ? 1 : 2) + (Q8 ? 512 : 0));
     const int fixed = W * 8 * NT * (HD + 2) * 4 + 2 * W * 16 + (4 * W + 1) * 4 + (2 * p.batch + 1) * 4;
     int n = 1;   // stages: as many as fit, 8 at most
-    while (!one_stage(HD, NT) && n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
+    while (!one_stage(Q8, HD, NT) && n < 8 && fixed + W * (n + 1) * (stage + 16) <= kPagedSmem) ++n;
     p.nstages = n;
     auto fn = paged_attn_kernel<BF16, Q8, HD, NT, W>;
     if (int r = set_smem_limit((const void*)fn, kPagedSmem)) return r;
@@ -1089,11 +1089,12 @@ template <bool BF16, bool Q8>
 int paged_attn_pick(PagedAttnParams& p, int hd, int grid, cudaStream_t s) {
     const bool two = p.chunk > 8;
     // Warps of a CTA.  Q8_0 is bound by instructions and takes as many as its registers allow (48
-    // sequences of 300 to 6000, 32 / 8 heads of 128: 8 warps 79.9 us, 12 77.5); 16-bit values
-    // need only enough in flight (64 sequences of 1 to 8192, heads of 128: 6 warps of two stages
-    // 177 us, 7 of one 168, 8 171, 9 175; heads of 64: 8 warps 87.1 us, 12 88.9).
+    // sequences of 300 to 6000, 32 / 8 heads of 128: 8 warps 79.9 us, 12 77.5; heads of 64: 8 86.1,
+    // 12 75.9, with one stage each 72.1 where the later 66.4 take three).  16-bit values need only
+    // enough in flight (64 sequences of 1 to 8192, heads of 128: 6 warps of two stages 177 us, 7 of one
+    // 168, 8 171, 9 175; 64 of 300 to 8000, heads of 64: 8 of three 87.4, 8 of one 83.0, 10 80.9, 12 81.7).
     if (hd == 64)
-        return two ? paged_attn_run<BF16, Q8, 64, 2, 8>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1, Q8 ? 12 : 8>(p, grid, s);
+        return two ? paged_attn_run<BF16, Q8, 64, 2, 8>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1, Q8 ? 12 : 10>(p, grid, s);
     if (two) return paged_attn_run<BF16, Q8, 128, 2, Q8 ? 8 : 4>(p, grid, s);
     return paged_attn_run<BF16, Q8, 128, 1, Q8 ? 12 : 7>(p, grid, s);
 }
