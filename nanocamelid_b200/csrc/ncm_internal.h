@@ -259,8 +259,9 @@ int num_sms();
 int set_smem_limit(const void* fn, int bytes);
 // Sets ncm_last_error() of the calling thread and returns `code` (engine.cu).
 int set_error(int code, const char* msg);
-// Whether p is device memory of the current device (0), else a message (paged.cu).
-const char* device_pointer_error(const void* p);
+// Null when all of p[0 .. n) are null or device memory of the current device, else a message
+// (paged.cu).
+const char* device_pointers_error(const void* const* p, int n);
 // The glibc expf exception table: at most kExpfTabEntries {key, value} pairs, kept in a
 // fixed in-library device array.
 constexpr uint32_t kExpfTabEntries = 1u << 20;

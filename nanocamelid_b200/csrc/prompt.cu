@@ -753,9 +753,7 @@ extern "C" ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const 
     }
     if (total_k == 0) { k = q; v = q; k_stride = q_stride; v_stride = q_stride; }   // never read: no row sees a key
     const void* check[] = {out, q, k, v, cu_q, cu_k, err};
-    for (const void* c : check)
-        if (c)
-            if (const char* e = device_pointer_error(c)) return bad(e);
+    if (const char* e = device_pointers_error(check, sizeof check / sizeof *check)) return bad(e);
     if (!encode_tiled_fn()) return set_error(NCM_ECUDA, "cuTensorMapEncodeTiled not available");
     PromptParams p;
     memset(&p, 0, sizeof p);
