@@ -93,7 +93,8 @@ __device__ __forceinline__ int place_of_token(const int* cu, const int* lengths,
         const int k = __popc(__ballot_sync(NCM_FULL, __ldg(cu + at) <= token));
         if (k == 32) return -1;
         lo += k * step;
-        n = min(step, n - k * step);                     // the answer is among these (the last probe's end is past the token)
+        // the answer is among these (the last probe's end is past the token)
+        n = min(step, n - k * step);
     }
     const int at = lo + min(lane, n - 1);
     const int first = __ldg(cu + at), end = __ldg(cu + at + 1), length = __ldg(lengths + at);
@@ -168,7 +169,8 @@ template <typename T>
 __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant__ AppendParams p) {
     const int token = blockIdx.x, hd = p.hd, per = hd >> 4;   // threads per head: 4 or 8
     const int all = (p.heads + 2 * p.kv_heads) * per;
-    const int part = threadIdx.x & (per - 1), lo = 8 * part, hi = (hd >> 1) + lo;   // the same for all of a thread's rows
+    // the same for all of a thread's rows
+    const int part = threadIdx.x & (per - 1), lo = 8 * part, hi = (hd >> 1) + lo;
     int off = 0, page = -1;
     float4 turn[4];                        // two (sin, cos) each, of the thread's eight pairs
     bool ready = false;
@@ -224,7 +226,8 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
             } else {          // pairs (2i, 2i + 1), the first rope_half of them
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    if ((((i < 8 ? lo : hi - 8) + i) >> 1) >= p.rope_half) continue;   // rope_half is even: two pairs at a time
+                    // rope_half is even: two pairs at a time
+                    if ((((i < 8 ? lo : hi - 8) + i) >> 1) >= p.rope_half) continue;
                     const float4 t = turn[i >> 2];
                     const float a = x[i], b = x[i + 1], c = x[i + 2], d = x[i + 3];
                     x[i] = a * t.y - b * t.x; x[i + 1] = a * t.x + b * t.y;
@@ -360,6 +363,8 @@ template <bool BF16>
 __device__ __forceinline__ void store_out(void* out, int64_t at, float4 v) {
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(pack2(BF16, v.x, v.y), pack2(BF16, v.z, v.w));
 }
+// 1 / sum; a row whose scores are all -infinity has nothing to divide and stays zero.
+__device__ __forceinline__ float inverse(float sum) { return sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f; }
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : ex2(m - top); }
 
 __host__ __device__ constexpr bool one_stage(bool q8, int hd, int nt) { return nt == 1 && (hd == 128 || !q8); }
@@ -491,7 +496,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         do { ++t.b; } while (t.b < p.batch && lens[t.b] == 0);
         t.n = t.b < p.batch ? (lens[t.b] + kUnit - 1) / kUnit : 1;
     };
-    const int box = p.box_rows, lbox = 31 - __clz(box), lnpg = 5 - lbox, npg = 1 << lnpg;   // boxes of a unit: one per page, or one of 32 rows
+    // boxes of a unit: one per page, or one of 32 rows
+    const int box = p.box_rows, lbox = 31 - __clz(box), lnpg = 5 - lbox, npg = 1 << lnpg;
     auto page_at = [&](const Place& t, int i) -> int {   // the page of box i < npg
         const int key = t.u * kUnit + i * box;
         if (i >= npg || key >= lens[t.b]) return -1;
@@ -572,17 +578,20 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
                     top = max_nan(top, __shfl_xor_sync(NCM_FULL, top, 1));
                     top = max_nan(top, __shfl_xor_sync(NCM_FULL, top, 2));
-                    const float inv = top > 0.0f && top < INFINITY ? 32512.0f / top : 0.0f;   // 127 * 256: high bytes fit
+                    // 127 * 256: high bytes fit
+                    const float inv = top > 0.0f && top < INFINITY ? 32512.0f / top : 0.0f;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint32_t v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[4 * i + e], inv, kIntBaseF));   // low 16 bits
+                        // low 16 bits
+                        for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[4 * i + e], inv, kIntBaseF));
                         const uint32_t v01 = __byte_perm(v[0], v[1], 0x5410), v23 = __byte_perm(v[2], v[3], 0x5410);
                         qf[2 * k][t][i] = __byte_perm(v01, v23, 0x7531);
                         qf[2 * k + 1][t][i] = __byte_perm(v01, v23, 0x6420);
                     }
-                    const float sc = top < INFINITY ? top * (1.0f / 32512.0f) : NAN;   // a query that is not finite: NaN
+                    // a query that is not finite: NaN
+                    const float sc = top < INFINITY ? top * (1.0f / 32512.0f) : NAN;
                     qs[k][t][0] = __shfl_sync(NCM_FULL, sc, 8 * c4);
                     qs[k][t][1] = __shfl_sync(NCM_FULL, sc, 8 * c4 + 4);
                 }
@@ -742,7 +751,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     for (int k = 0; k < KS; ++k) { o[k][t][j] *= a; o[k][t][j + 2] *= a; }
                 }
         }
-        if (ONE && fetched < count) issue(f, fpage, stage, true, false);   // all lanes have their scores (the vote): K has been read
+        // all lanes have their scores (the vote): K has been read
+        if (ONE && fetched < count) issue(f, fpage, stage, true, false);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -872,7 +882,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int head = t * 8 + 2 * c4 + (j & 1);
-                        const float inv = 1.0f / l[t][j & 1];
+                        const float inv = inverse(l[t][j & 1]);
                         if (head < heads)
 #pragma unroll
                             for (int k = 0; k < KS; ++k)
@@ -948,7 +958,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             }
             if (d >= HD) continue;
             if (inside) {
-                const float inv = 1.0f / sum;
+                const float inv = inverse(sum);
                 store_out<BF16>(p.out, out_at + head * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
             } else {
                 *reinterpret_cast<float4*>(rows + head * HD + d) = acc;
@@ -993,7 +1003,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                             acc.z = fmaf(w, v[i].z, acc.z); acc.w = fmaf(w, v[i].w, acc.w);
                             sum = fmaf(w, ml[i].y, sum);
                         }
-                        const float inv = 1.0f / sum;
+                        const float inv = inverse(sum);
                         store_out<BF16>(p.out, out_at + head * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
                     }
                     e = e1;
@@ -1013,7 +1023,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(NCM_FULL, sum, x);
-                    const float inv = 1.0f / sum;
+                    const float inv = inverse(sum);
                     for (int i = lane; i < np; i += 32) weights[i * GH + head] *= inv;
                 }
                 __syncthreads();
@@ -1235,7 +1245,8 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     p.part = (float*)((char*)workspace + 4096);
     p.err = err;
     // positions in the row of units, padded to pieces, fit 32 bits
-    const int64_t most = ((int64_t)table_width * kv->page_size / kUnit + 1 + 48) * kv->kv_heads * p.nchunk;   // 4 * 12: a piece
+    // 4 * 12: a piece
+    const int64_t most = ((int64_t)table_width * kv->page_size / kUnit + 1 + 48) * kv->kv_heads * p.nchunk;
     const int step = (int)std::min<int64_t>(kPagedBatch, (int64_t)0x7fff0000 / most);
     if (step < 1) return set_error(NCM_EUNSUPPORTED, "a sequence's pages hold too many tokens for so many heads");
     cudaStream_t s = (cudaStream_t)stream;

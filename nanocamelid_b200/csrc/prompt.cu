@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     uint64_t *empty = full + NST, *edge = empty + NST, *q_full = edge + NST, *q_empty = q_full + 1, *s_ready = q_empty + 1,
              *p_ready = s_ready + 2, *pv_done = p_ready + 4, *o_ready = pv_done + 2,   // [x], [2 x + h], [x], [x]
              *n_full = o_ready + 2, *n_empty = n_full + 2;
-    uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::kWords);   // [0] TMEM address, [8..16) items with odd V, [16..28) sums
+    // [0] TMEM address, [8..16) items with odd V, [16..28) sums
+    uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::kWords);
     int* prefix = reinterpret_cast<int*>(smem + L::kPrefix);
     const int tid = threadIdx.x, warp = __shfl_sync(NCM_FULL, tid >> 5, 0), lane = tid & 31;
     bool ok = true;
@@ -588,7 +589,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                     if (over && now < INFINITY) top = now;
                     sum *= a;
                     if (!(now < INFINITY)) sum = NAN;
-                    if (u > 0) {   // O is at rest once the last unit's products are complete (those before it are: S is here)
+                    // O is at rest once the last unit's products are complete (those before it are: S is here)
+                    if (u > 0) {
                         if (!wait_all(pv_done + x, (handed - 1) & 1)) break;
                         fence_after();
 #pragma unroll 1
@@ -640,7 +642,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 fence_after();
             }
             const bool odd = words[8 + (it & 7)] == it + 1;
-            const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;   // a row without keys: zeros
+            // A row without keys, or with none that scores above -infinity: zeros (what ex2_poly made of
+            // such scores is in its sum).  The sum is at least one otherwise, or NaN.
+            const float inv = top == -INFINITY && sum == sum ? 0.0f : 1.0f / sum;
             // Rows leave through shared memory, 32 columns at a time: four lanes then write 64
             // bytes of a row, where one lane per row would touch 32 lines with every store.
             uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)(t.q0 + at) * p.out_stride + (int64_t)(t.head * p.group + member) * HD;

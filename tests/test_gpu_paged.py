@@ -261,6 +261,21 @@ def test_attention_nan_in_a_key_stays_in_its_sequence(ncm, cuda):
         assert bool(((out[i].double() - ref).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("n", [5, 40, 3000, 40000])
+def test_attention_with_all_scores_minus_infinity(ncm, cuda, n):
+    """Keys of -infinity in one sequence: its rows are zeros, as if it had no keys; whole segments,
+    parts joined in one CTA, and parts joined over few and many."""
+    heads, kvh, hd = 8, 2, 64
+    c = Cache(ncm, "bf16", kvh, hd, 64, [n, 50], seed=13).fill()
+    pages = c.table[0, :-(-n // 64)].long()
+    c.k[pages] = float("-inf")
+    q = torch.rand((2, heads, hd), generator=c.g, device="cuda").bfloat16() + 1
+    out = attend(ncm, c, q, int32([n, 50]), heads, "bf16")
+    assert bool((out[0] == 0).all())
+    ref, tol = attend64(q[1], c.rows("k", 1, 50), c.rows("v", 1, 50), 0.125, "bf16", hd)
+    assert bool(((out[1].double() - ref).abs() <= tol).all())
+
+
 def test_attention_in_graphs_and_streams(ncm, cuda):
     """Two captured graphs that share a workspace, replayed in turn with new lengths and inputs."""
     heads, kvh, hd = 16, 2, 128

@@ -149,6 +149,17 @@ def test_prompt_hidden_values_do_not_matter(ncm, cuda, kind, heads, kvh, hd):
         assert torch.equal(out[:at], good[:at]) and torch.equal(out[270:], good[270:]) and bool(out[at:270].isnan().all())
 
 
+def test_prompt_with_all_scores_minus_infinity(ncm, cuda):
+    """Keys of -infinity in the middle sequence: zeros there, the others as they were."""
+    lens = [60, 150, 40]
+    q, k, v = inputs(lens, lens, 4, 2, 64, "bf16", seed=9)
+    q, cu = q.abs() + 1, int32(starts(lens))
+    good = attend(ncm, q, k, v, cu, cu, "bf16", True)
+    k[60:210] = float("-inf")
+    out = attend(ncm, q, k, v, cu, cu, "bf16", True)
+    assert bool((out[60:210] == 0).all()) and torch.equal(out[:60], good[:60]) and torch.equal(out[210:], good[210:])
+
+
 def test_prompt_strides(ncm, cuda):
     """q, k and v as slices of one projection's rows, out rows apart."""
     lens, heads, kvh, hd = [40, 333], 8, 2, 64
