@@ -969,15 +969,17 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             // The CTA that stores its part last joins them all, in the CTAs' order: the result
             // does not depend on which one that is.  Nobody waits.
             const int i0 = sb / share, i1 = (se - 1) / share;
-            __threadfence();
+            // (the barriers carry the other threads' stores and loads over one thread's release
+            // and acquire)
             __syncthreads();
             if (tid == 0) {
-                sums[4 * W] = (int)atomicAdd(p.counters + i0, 1u) == i1 - i0;
+                unsigned before;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + i0) : "memory");
+                sums[4 * W] = (int)before == i1 - i0;
                 if (sums[4 * W]) p.counters[i0] = 0;
             }
             __syncthreads();
             if (sums[4 * W]) {
-                __threadfence();
                 const int np = i1 - i0 + 1;
                 auto part_of = [&](int i) { return (int64_t)(2 * (i0 + i) + (i == 0 ? 1 : 0)); };
                 if (np <= 8) {   // one round of loads
