@@ -175,9 +175,10 @@ ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, const void* q, 
  * that share a page table row's contents.  table_width * page_size <= 2^22; a longer length
  * is cut there and a page id out of range reads as zeros (both NCM_DEVICE_BAD_ARG).
  * scale 0 means 1 / sqrt(head_dim).  Softmax and sums are f32; p is rounded to q_type.  Over
- * Q8_0 a query is taken as a multiple of its block's largest value / 32512 and p times the
- * value's scale as a multiple of the largest such product among 32 keys / 65534.  The result
- * does not depend on the order in which the parts of a long sequence finish.
+ * Q8_0 a query is taken as a multiple of its block's largest value / 32512, and p times the
+ * value's scale as a multiple of at most 1 / 65000 of the largest such product among 32 keys (from
+ * a multiple of 32 on).  The result does not depend on the order in which the parts of a long
+ * sequence finish.
  * workspace: at least ncm_paged_attention_workspace bytes, zeroed once before its first use
  * (each call leaves its counters zero again, unless it ends with NCM_DEVICE_TIMEOUT); calls
  * that can overlap on the GPU need one each, calls in stream order, graph replays among

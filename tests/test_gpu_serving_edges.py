@@ -1,0 +1,50 @@
+"""The batched serving operators at the ends of their ranges, against plain forms in 64 bits.
+
+Tolerances are those of test_gpu_paged and test_gpu_prompt but for the terms that the tests state.
+Over Q8_0 include/ncm.h has each weight, p times scale, as a multiple of at most 1/65000 of the
+largest such product among 32 keys (from a multiple of 32 on): it is off by 1/130000 of that, times a
+value of at most 127, for each of the 32."""
+import pytest
+import torch
+
+from test_gpu_paged import DT, U, Cache, attend, attend64 as attend_one, int32
+
+pytestmark = pytest.mark.gpu
+
+
+def attend_q8(q, k, v, v_scales, scale, qkind):
+    """attend_one over a Q8_0 cache, with the term of the weights by their products."""
+    heads, hd = q.shape
+    g = heads // k.shape[1]
+    o, _ = attend_one(q, k, v, scale, qkind, hd)
+    kr, vr = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    w = torch.softmax(torch.einsum("hd,nhd->hn", q.double(), kr) * scale, -1)
+    a = torch.einsum("hn,nhd->hd", w, vr.abs())
+    top = (torch.einsum("hd,nhd->hn", q.double().abs(), kr.abs()) * scale).amax(-1)[:, None]
+    step = q.double().abs().unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1) / 65024
+    e = 2 * (2.0 ** -24 * (hd + 4) * top + 2.0 ** -21) + k.shape[0] * 2.0 ** -24
+    e = e + 2 * (torch.einsum("hd,nhd->hn", step, kr.abs()) * scale).amax(-1)[:, None]
+    prod = w.T[:, :, None] * v_scales.double().repeat_interleave(g, 1)                                      # [n, heads, hd / 32]
+    prod = torch.nn.functional.pad(prod, (0, 0, 0, 0, 0, -k.shape[0] % 32)).unflatten(0, (-1, 32)).amax(1)  # [units, heads, hd / 32]
+    return o, U[qkind] * o.abs() + e * a * (1 + U[qkind]) + prod.sum(0).repeat_interleave(32, -1) * (32 * 127 / 130000)
+
+
+@pytest.mark.parametrize("qkind", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 64), (8, 2, 128), (12, 1, 64), (24, 2, 128)])
+@pytest.mark.parametrize("lengths", [[32, 77, 3000], [1000] * 40, [20000]])
+@pytest.mark.parametrize("less", [1, 100, 1000])
+def test_q8_weights_of_a_sink(ncm, cuda, qkind, heads, kvh, hd, lengths, less):
+    """One key takes nearly all weight and its value is small, as the first token of a text does."""
+    c = Cache(ncm, "q8_0", kvh, hd, 16, lengths, seed=hd + less).fill()
+    q = (torch.rand((len(lengths), heads, hd), generator=c.g, device="cuda") + 0.5).to(DT[qkind])
+    for i, n in enumerate(lengths):
+        at = 5 if i % 2 else n - 1 - n // 3
+        page, off = c.table[i, at // 16].item(), at % 16
+        c.k[page, :, off] = 100
+        c.ks[page, :, off] = 0.011 if hd == 128 else 0.016    # a score of about 12 over the others': 2^-18 and up of its weight
+        c.vs[page, :, off] = torch.as_tensor(0.01 / less).half()
+    out = attend(ncm, c, q, int32(lengths), heads, qkind)
+    for i, n in enumerate(lengths):
+        ref, tol = attend_q8(q[i], c.rows("k", i, n), c.rows("v", i, n), c.rows("v_scales", i, n), hd ** -0.5, qkind)
+        off = (out[i].double() - ref).abs()
+        assert bool((off <= tol).all()), (i, n, float((off / tol).max()), float((off / ref.abs().mean()).max()))
