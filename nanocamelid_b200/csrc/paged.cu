@@ -342,9 +342,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 template <bool BF16> __device__ __forceinline__ float2 widen2(uint32_t w) {
@@ -808,7 +808,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             // largest p times the largest scale (69.5 us where this takes 70.9: 48 sequences of 300
             // to 6000, 32 / 8 heads of 128) a key of large p and small scale would take the others'
             // bits.  The largest is rounded up to bf16's eight bits, two heads to a register for the
-            // shuffles: each weight is off by 1 / 130000 of it at most.
+            // shuffles: each weight is off by 1 / 130000 of it at most.  A NaN among the products
+            // becomes the largest, and with it the unit's share of the output.
             const int swz = HD == 128 ? (lane & 7) : ((lane >> 1) & 3);
             float sv[4][NB];
             uint32_t top2[NB][NT];
@@ -820,8 +821,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     float v[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
-                        v[j] = fmaxf(fmaxf(s[0][t][j] * sv[0][k], s[0][t][j + 2] * sv[1][k]),
-                                     fmaxf(s[1][t][j] * sv[2][k], s[1][t][j + 2] * sv[3][k])) * (1.0f + 0x1p-8f);
+                        v[j] = max_nan(max_nan(s[0][t][j] * sv[0][k], s[0][t][j + 2] * sv[1][k]),
+                                       max_nan(s[1][t][j] * sv[2][k], s[1][t][j + 2] * sv[3][k])) * (1.0f + 0x1p-8f);
                     top2[k][t] = pack2(true, v[0], v[1]);
                 }
 #pragma unroll
@@ -829,7 +830,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
 #pragma unroll
                 for (int k = 0; k < NB; ++k)
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) top2[k][t] = max_bf16x2(top2[k][t], __shfl_xor_sync(NCM_FULL, top2[k][t], x));
+                    for (int t = 0; t < NT; ++t) top2[k][t] = max_nan_bf16x2(top2[k][t], __shfl_xor_sync(NCM_FULL, top2[k][t], x));
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
                 uint32_t hi[NT][2], lo[NT][2];
@@ -839,7 +840,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     float r[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float v = fmaxf(__uint_as_float(j ? top2[k][t] & 0xffff0000u : top2[k][t] << 16), 0x1p-84f);
+                        const float v = max_nan(__uint_as_float(j ? top2[k][t] & 0xffff0000u : top2[k][t] << 16), 0x1p-84f);
                         r[j] = __fdividef(65534.0f, v);
                         step[t][j] = v * (1.0f / 65534.0f);
                     }

@@ -48,3 +48,36 @@ def test_q8_weights_of_a_sink(ncm, cuda, qkind, heads, kvh, hd, lengths, less):
         ref, tol = attend_q8(q[i], c.rows("k", i, n), c.rows("v", i, n), c.rows("v_scales", i, n), hd ** -0.5, qkind)
         off = (out[i].double() - ref).abs()
         assert bool((off <= tol).all()), (i, n, float((off / tol).max()), float((off / ref.abs().mean()).max()))
+
+
+@pytest.mark.parametrize("n", [5, 40, 3000, 40000])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_q8_not_finite(ncm, cuda, n, hd):
+    """Scores that are all -infinity give zeros; a NaN in a key's or a value's scale or in a query
+    reaches its outputs and no others."""
+    heads, kvh = 8, 2
+    c = Cache(ncm, "q8_0", kvh, hd, 64, [n, 50], seed=13).fill()
+    pages, lengths = c.table[0, :-(-n // 64)].long(), int32([n, 50])
+    q = torch.rand((2, heads, hd), generator=c.g, device="cuda").bfloat16() + 1
+    good = attend(ncm, c, q, lengths, heads, "bf16")
+    assert bool(good.isfinite().all())
+    page, off = c.table[0, (n - 1) // 2 // 64].item(), (n - 1) // 2 % 64
+    for plane in (c.ks, c.vs):
+        keep = plane[page, 1, off, 1].clone()
+        plane[page, 1, off, 1] = float("nan")
+        out = attend(ncm, c, q, lengths, heads, "bf16")
+        plane[page, 1, off, 1] = keep
+        assert torch.equal(out[1], good[1]) and torch.equal(out[0, :4], good[0, :4])
+        block = out[0, 4:] if plane is c.ks else out[0, 4:, 32:64]
+        assert bool(block.isnan().all())
+        if plane is c.vs:
+            assert torch.equal(out[0, 4:, :32], good[0, 4:, :32]) and torch.equal(out[0, 4:, 64:], good[0, 4:, 64:])
+    bad = q.clone()
+    bad[0, 2, 7] = float("nan")
+    out = attend(ncm, c, bad, lengths, heads, "bf16")
+    rest = [0, 1, 3, 4, 5, 6, 7]
+    assert bool(out[0, 2].isnan().all()) and torch.equal(out[0, rest], good[0, rest]) and torch.equal(out[1], good[1])
+    c.k[pages] = -1
+    c.ks[pages] = float("inf")
+    out = attend(ncm, c, q, lengths, heads, "bf16")
+    assert bool((out[0] == 0).all()) and torch.equal(out[1], good[1])
