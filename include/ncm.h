@@ -174,7 +174,8 @@ ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, const void* q, 
  * Several rows of one sequence (a speculative batch) are passed as sequences of their own
  * that share a page table row's contents.  table_width * page_size <= 2^22; a longer length
  * is cut there and a page id out of range reads as zeros (both NCM_DEVICE_BAD_ARG).
- * scale 0 means 1 / sqrt(head_dim).  Softmax and sums are f32; p is rounded to q_type.  Over
+ * scale 0 means 1 / sqrt(head_dim).  Softmax and sums are f32; p, the largest of which
+ * is at least 1, is rounded to q_type (times 2^7 in F16, so that one below 2^-21 is off by 2^-32).  Over
  * Q8_0 a query is taken as a multiple of its block's largest value / 32512, and p times the
  * value's scale as a multiple of at most 1 / 65000 of the largest such product among 32 keys (from
  * a multiple of 32 on).  The result does not depend on the order in which the parts of a long
@@ -201,7 +202,8 @@ ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_st
  * or BF16), tokens *_stride elements apart (0: dense), 16-byte aligned; head_dim 64 or 128, at
  * most 128 query heads to a key-value head; out may not overlap an input.  scale 0 means
  * 1 / sqrt(head_dim).  cu_* entries that fall or lie past total_q / total_k are cut to the range
- * (NCM_DEVICE_BAD_ARG).  Runs on tcgen05; p is rounded to `type`, sums are f32. */
+ * (NCM_DEVICE_BAD_ARG).  Runs on tcgen05; p is rounded to `type` as by
+ * ncm_paged_attention, sums are f32. */
 ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k,
                                 int64_t k_stride, const void* v, int64_t v_stride, int type, int total_q, int total_k,
                                 int batch, int heads, int kv_heads, int head_dim, const int* cu_q, const int* cu_k,

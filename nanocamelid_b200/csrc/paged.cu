@@ -390,6 +390,9 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     constexpr int STAGE = 2 * (KB + SB);
     constexpr int KS = HD / 16, NB = HD / 32;
     constexpr bool ONE = one_stage(Q8, HD, NT);                      // K and V of a unit are then fetched apart
+    // p and its sums times 2^7 where p is rounded to f16: 2^15 at most then, and what is below 2^-14 of
+    // the largest, where f16's steps no longer shrink, is held 2^7 times finer.
+    constexpr float kLift = BF16 || Q8 ? 0.0f : 7.0f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c4 = lane & 3, r8 = lane >> 2;
     const int nst = p.nstages;
 
@@ -762,7 +765,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float mm = m[t][j & 1] == -INFINITY ? 0.0f : m[t][j & 1];
+                const float mm = m[t][j & 1] == -INFINITY ? 0.0f : m[t][j & 1] - kLift;
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
                     s[a][t][j] = ex2(fmaf(s[a][t][j], p.scale_log2, -mm));

@@ -541,6 +541,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     } else {
         // ---- softmax, one row per thread
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // p and its sum times 2^7 in f16: 2^15 at most then, and what is below 2^-14 of the largest, where
+        // f16's steps no longer shrink, is held 2^7 times finer.
+        constexpr float kLift = BF16 ? 0.0f : 7.0f;
         const int x = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // 32 lanes per warp, in bits 16 and up
         const uint32_t s_at = tmem + x * 128 + lanes, o_at = tmem + 256 + x * 128 + lanes;
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                         }
                     }
                 }
-                const float shift = top == -INFINITY ? 0.0f : -top;
+                const float shift = top == -INFINITY ? 0.0f : kLift - top;
                 const uint64_t scale2 = two(p.scale_log2, p.scale_log2), shift2 = two(shift, shift);
                 uint64_t l0 = 0, l1 = 0;
                 // p of 32 columns; with a mask by ex2 alone, which gives 0 where it hides

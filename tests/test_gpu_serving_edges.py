@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from test_gpu_paged import DT, U, Cache, attend, attend64 as attend_one, int32
+from test_gpu_prompt import E, attend as attend_prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,28 @@ def test_q8_not_finite(ncm, cuda, n, hd):
     c.ks[pages] = float("inf")
     out = attend(ncm, c, q, lengths, heads, "bf16")
     assert bool((out[0] == 0).all()) and torch.equal(out[1], good[1])
+
+
+@pytest.mark.parametrize("less", [12.5, 4.5, 1.5, 0.45])
+def test_f16_many_small_weights(ncm, cuda, less):
+    """A key of weight one and 2^18 of `less` x 2^-24 each: together they matter, and each lies among
+    f16's subnormal numbers or below them.  Held times 2^7, one below 2^-21 is off by 2^-32, half a
+    step of those numbers."""
+    n, hd, heads = 1 << 18, 64, 8
+    k, v = torch.zeros((n, hd), device="cuda").half(), torch.ones((n, hd), device="cuda").half()
+    at = 12345
+    q = torch.ones((1, heads, hd), device="cuda").half()
+    # scale * q.k = ln 2 * (24 - log2 less), to f16's precision; the sink's value is zero
+    k[at], v[at] = (24 - torch.log2(torch.tensor(less)).item()) * 0.6931471805599453 / 8.0, 0.0
+    c = Cache(ncm, "f16", 1, hd, 64, [n], seed=1)
+    order = c.table[0].long()
+    c.k[order, 0], c.v[order, 0] = k.view(-1, 64, hd), v.view(-1, 64, hd)
+    s = q[0, 0].double() @ k.double().T * 0.125
+    w = torch.softmax(s, -1)
+    o = (w @ v.double())[0].item()
+    e = 2 * (2.0 ** -24 * (hd + 4) * s.abs().max().item() + 2.0 ** -21) + n * 2.0 ** -24 + E["f16"]
+    tol = U["f16"] * o + (U["f16"] + e) * o * (1 + U["f16"]) + n * 2.0 ** -32
+    out = attend(ncm, c, q, int32([n]), heads, "f16")
+    assert bool(((out.double() - o).abs() <= tol).all()), (float(out[0, 0, 0]), o, tol)
+    out = attend_prompt(ncm, q, k[:, None], v[:, None], int32([0, 1]), int32([0, n]), "f16", True)
+    assert bool(((out.double() - o).abs() <= tol).all()), (float(out[0, 0, 0]), o, tol)
