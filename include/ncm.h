@@ -168,7 +168,8 @@ ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, const void* q, 
 /* Attention of one new token per sequence over a paged cache:
  *   out[s][h] = sum_j softmax_j(scale * q[s][h] . K_j) V_j over j < lengths[s],
  * query head h reading key-value head h / (heads / kv_heads).  A sequence of length 0 or less
- * gets a row of zeros, as does one whose scores are all -infinity; rows of the cache behind the length count for nothing, whatever they hold.
+ * gets a row of zeros, as does one whose scores are all -infinity, whatever its values are; rows
+ * of the cache behind the length count for nothing, whatever they hold.
  * q and out are of q_type (F16 or BF16: the cache's type, either one over Q8_0), rows
  * q_stride / out_stride elements apart (0: dense), 16-byte aligned; out may not overlap q.
  * Several rows of one sequence (a speculative batch) are passed as sequences of their own
@@ -196,8 +197,9 @@ ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_st
  *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j
  * over the sequence's keys; with causal != 0 its last query sees its last key, the one before
  * one key less, and so on, so that a chunk of a prompt can be passed with all keys before it.
- * A query that sees no key, or whose scores are all -infinity, gets zeros.  Keys that a row does not see do not change it, NaN and
- * infinities among them.  Rows of out that belong to no sequence are left alone.
+ * A query that sees no key, or whose scores are all -infinity, gets zeros, whatever the values are.
+ * Keys that a row does not see do not change it, NaN and infinities among them.  Rows of out that
+ * belong to no sequence are left alone.
  * q and out: [total_q][heads][head_dim], k and v: [total_k][kv_heads][head_dim], of `type` (F16
  * or BF16), tokens *_stride elements apart (0: dense), 16-byte aligned; head_dim 64 or 128, at
  * most 128 query heads to a key-value head; out may not overlap an input.  scale 0 means

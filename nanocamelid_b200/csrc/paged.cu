@@ -370,6 +370,11 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, float4 v) {
 }
 // 1 / sum; a row whose scores are all -infinity has nothing to divide and stays zero.
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f; }
+// (also where its values are not finite, whose products with zero are not zero)
+__device__ __forceinline__ float scaled(float v, float inv) { return inv == 0.0f ? 0.0f : v * inv; }
+__device__ __forceinline__ float4 scaled(float4 v, float inv) {
+    return make_float4(scaled(v.x, inv), scaled(v.y, inv), scaled(v.z, inv), scaled(v.w, inv));
+}
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : ex2(m - top); }
 
 __host__ __device__ constexpr bool one_stage(bool q8, int hd, int nt) { return nt == 1 && (hd == 128 || !q8); }
@@ -903,7 +908,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                         if (head < heads)
 #pragma unroll
                             for (int k = 0; k < KS; ++k)
-                                out[head * HD + d_of(k, j)] = (uint16_t)pack2(BF16, o[k][t][j] * inv, 0.0f);
+                                out[head * HD + d_of(k, j)] = (uint16_t)pack2(BF16, scaled(o[k][t][j], inv), 0.0f);
                     }
             } else {
                 const bool at_end = i + 1 == count;
@@ -932,7 +937,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
     __syncthreads();
 
     // ---- the CTA's parts, joined where they are of one segment
-    float* weights = last_ml + W * GH * 2;   // [parts][GH] of the join over CTAs
+    float* weights = last_ml + W * GH * 2;   // [parts + 1][GH] of the join over CTAs
     for (int e = 0; e < 2 * W;) {
         const int4 seg = *reinterpret_cast<const int4*>(ent + 4 * e);
         if (seg.x < 0) { ++e; continue; }
@@ -976,7 +981,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
             if (d >= HD) continue;
             if (inside) {
                 const float inv = inverse(sum);
-                store_out<BF16>(p.out, out_at + head * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+                store_out<BF16>(p.out, out_at + head * HD + d, scaled(acc, inv));
             } else {
                 *reinterpret_cast<float4*>(rows + head * HD + d) = acc;
                 if (d == 0) *reinterpret_cast<float2*>(mls + ((int64_t)(2 * blockIdx.x + slot) * p.chunk + head) * 2) = make_float2(top, sum);
@@ -1023,12 +1028,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                             sum = fmaf(w, ml[i].y, sum);
                         }
                         const float inv = inverse(sum);
-                        store_out<BF16>(p.out, out_at + head * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+                        store_out<BF16>(p.out, out_at + head * HD + d, scaled(acc, inv));
                     }
                     e = e1;
                     continue;
                 }
-                // weights of the parts, one warp per head in turn; their joint sum is folded in
+                // weights of the parts, one warp per head in turn, and the inverse of their joint sum
                 for (int head = warp; head < heads; head += W) {
                     float top = -INFINITY, sum = 0.0f;
                     for (int i = lane; i < np; i += 32) top = fmaxf(top, __ldcg(mls + (part_of(i) * p.chunk + head) * 2));
@@ -1042,8 +1047,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(NCM_FULL, sum, x);
-                    const float inv = inverse(sum);
-                    for (int i = lane; i < np; i += 32) weights[i * GH + head] *= inv;
+                    if (lane == 0) weights[np * GH + head] = inverse(sum);
                 }
                 __syncthreads();
                 for (int x = tid; x < heads * (HD / 4); x += W * 32) {
@@ -1056,7 +1060,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
                         acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
                         acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
                     }
-                    store_out<BF16>(p.out, out_at + head * HD + d, acc);
+                    store_out<BF16>(p.out, out_at + head * HD + d, scaled(acc, weights[np * GH + head]));
                 }
                 __syncthreads();
             }

@@ -677,6 +677,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                             if (not_finite<BF16>(h)) o[i] = __float_as_uint(__uint_as_float(o[i]) + widen<BF16>(h));
                         }
                 }
+                // (zero times a value that is not finite is not zero)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = inv == 0.0f ? 0u : o[i];
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {

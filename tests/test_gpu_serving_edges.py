@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_gpu_paged import DT, U, Cache, attend, attend64 as attend_one, int32
-from test_gpu_prompt import E, attend as attend_prompt
+from test_gpu_prompt import E, attend as attend_prompt, inputs, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,33 @@ def test_f16_many_small_weights(ncm, cuda, less):
     assert bool(((out.double() - o).abs() <= tol).all()), (float(out[0, 0, 0]), o, tol)
     out = attend_prompt(ncm, q, k[:, None], v[:, None], int32([0, 1]), int32([0, n]), "f16", True)
     assert bool(((out.double() - o).abs() <= tol).all()), (float(out[0, 0, 0]), o, tol)
+
+
+@pytest.mark.parametrize("n", [5, 40, 3000, 40000])
+def test_all_scores_minus_infinity_over_values_that_are_not_finite(ncm, cuda, n):
+    """Zeros, whatever the values hold: whole segments, parts joined in a CTA and over few and many."""
+    heads, kvh, hd = 8, 2, 64
+    for kind in ("bf16", "f16"):
+        c = Cache(ncm, kind, kvh, hd, 64, [n, 50], seed=13).fill()
+        q = torch.rand((2, heads, hd), generator=c.g, device="cuda").to(DT[kind]) + 1
+        good = attend(ncm, c, q, int32([n, 50]), heads, kind)
+        pages = c.table[0, :-(-n // 64)].long()
+        c.k[pages], c.v[pages] = float("-inf"), float("inf")
+        c.v[pages, :, 3] = float("nan")
+        out = attend(ncm, c, q, int32([n, 50]), heads, kind)
+        assert bool((out[0] == 0).all()) and torch.equal(out[1], good[1])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_prompt_all_scores_minus_infinity_over_values_that_are_not_finite(ncm, cuda, kind):
+    lens = [60, 150, 400, 40]
+    q, k, v = inputs(lens, lens, 4, 2, 64, kind, seed=9)
+    q, cu = q.abs() + 1, int32(starts(lens))
+    good = attend_prompt(ncm, q, k, v, cu, cu, kind, True)
+    k[60:610], v[60:610] = float("-inf"), float("inf")
+    v[60:610:7] = float("nan")
+    for causal in (True, False):
+        out = attend_prompt(ncm, q, k, v, cu, cu, kind, causal)
+        assert bool((out[60:610] == 0).all())
+        if causal:
+            assert torch.equal(out[:60], good[:60]) and torch.equal(out[610:], good[610:])
