@@ -203,7 +203,8 @@ ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_st
  * q and out: [total_q][heads][head_dim], k and v: [total_k][kv_heads][head_dim], of `type` (F16
  * or BF16), tokens *_stride elements apart (0: dense), 16-byte aligned; head_dim 64 or 128, at
  * most 128 query heads to a key-value head; out may not overlap an input.  scale 0 means
- * 1 / sqrt(head_dim).  cu_* entries that fall or lie past total_q / total_k are cut to the range
+ * 1 / sqrt(head_dim).  An entry of cu_q below an earlier one counts as that one, an entry of
+ * cu_* below 0 or past total_q / total_k as that border, and where cu_k falls a sequence has no keys
  * (NCM_DEVICE_BAD_ARG).  Runs on tcgen05; p is rounded to `type` as by
  * ncm_paged_attention, sums are f32. */
 ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k,

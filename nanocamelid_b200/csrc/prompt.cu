@@ -54,6 +54,7 @@ struct alignas(64) PromptParams {
     int64_t out_stride, v_stride;        // elements between tokens
     const int *cu_q, *cu_k;
     int batch, kv_heads, group, tokens;  // tokens: of a tile, 128 / group
+    int before;                          // sequences of earlier launches, whose starts lie before cu_q
     int total_q, total_k, causal;
     float scale_log2;
     int* err;
@@ -233,10 +234,9 @@ __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix
     }
     t.b = lo;
     const int2 q = make_int2(cu_q[lo], cu_q[lo + 1]), k = make_int2(cu_k[lo], cu_k[lo + 1]);
-    t.q0 = min(max(q.x, 0), p.total_q); t.nq = min(max(q.y, t.q0), p.total_q) - t.q0;
+    t.q0 = q.x; t.nq = q.y - q.x;
     t.k0 = min(max(k.x, 0), p.total_k); t.nk = min(max(k.y, t.k0), p.total_k) - t.k0;
     t.t0 = (block - prefix[lo]) * 2 * p.tokens;
-    if (t.t0 < 0) t.t0 = t.nq;   // sums that ran over, from cu_q entries out of order: an item without rows
     t.shift = t.nk - t.nq;
     int least = t.nk;                                             // keys that every row sees
 #pragma unroll
@@ -318,27 +318,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
     if (tid < 8) words[8 + tid] = 0;
     {
         const int per = (p.batch + kPromptThreads - 1) / kPromptThreads, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
-        int sum = 0;
+        int* cu_q = prefix + p.batch + 1;
+        auto blocks_of = [&](int rows) { return (rows + 2 * p.tokens - 1) / (2 * p.tokens); };
+        int sum = 0, run;
+        bool falls = false;   // starts in q out of order or range
         for (int b = b0; b < b1; ++b) {
             const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1), k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
-            if (blockIdx.x == 0 && (q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k))
-                set_dev_error(p.err, NCM_DEVERR_BAD_ARG);
-            const int at = min(max(q0, 0), p.total_q), n = min(max(q1, at), p.total_q) - at;
-            prefix[b + 1] = (n + 2 * p.tokens - 1) / (2 * p.tokens);
+            const bool bad_q = q0 < 0 || q1 < q0 || q1 > p.total_q;
+            if (blockIdx.x == 0 && (bad_q || k0 < 0 || k1 < k0 || k1 > p.total_k)) set_dev_error(p.err, NCM_DEVERR_BAD_ARG);
+            falls |= bad_q;
+            prefix[b + 1] = bad_q ? 0 : blocks_of(q1 - q0);
             sum += prefix[b + 1];
         }
         for (int b = tid; b <= p.batch; b += kPromptThreads) {
-            prefix[p.batch + 1 + b] = __ldg(p.cu_q + b);
+            cu_q[b] = __ldg(p.cu_q + b);
             prefix[2 * (p.batch + 1) + b] = __ldg(p.cu_k + b);
         }
-        int run = sum;
+        for (int b = tid; b < p.before; b += kPromptThreads) falls |= __ldg(p.cu_q + b - p.before) > __ldg(p.cu_q);
+        while (true) {
+            run = sum;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(NCM_FULL, run, o);
-            if (lane >= o) run += v;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(NCM_FULL, run, o);
+                if (lane >= o) run += v;
+            }
+            if (lane == 31) words[16 + warp] = run;
+            if (!__syncthreads_or(falls)) break;
+            // Each start counts as the largest up to it, within the range: no row has two sequences, and there
+            // are no more blocks than the grid was made for.
+            if (warp == 0) {
+                int top = 0;
+                for (int b = lane; b < p.before; b += 32) top = max(top, __ldg(p.cu_q + b - p.before));
+                top = __reduce_max_sync(NCM_FULL, top);
+                for (int at = 0; at <= p.batch; at += 32) {
+                    int v = at + lane <= p.batch ? max(top, cu_q[at + lane]) : top;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int w = __shfl_up_sync(NCM_FULL, v, o);
+                        if (lane >= o) v = max(v, w);
+                    }
+                    if (at + lane <= p.batch) cu_q[at + lane] = min(v, p.total_q);
+                    top = __shfl_sync(NCM_FULL, v, 31);
+                }
+            }
+            __syncthreads();
+            sum = 0;
+            for (int b = b0; b < b1; ++b) {
+                prefix[b + 1] = blocks_of(cu_q[b + 1] - cu_q[b]);
+                sum += prefix[b + 1];
+            }
+            falls = false;
         }
-        if (lane == 31) words[16 + warp] = run;
-        __syncthreads();
         run -= sum;
         for (int w = 0; w < warp; ++w) run += words[16 + w];
         if (tid == 0) prefix[0] = 0;
@@ -780,6 +810,7 @@ extern "C" ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const 
     cudaStream_t s = (cudaStream_t)stream;
     for (int b = 0; b < batch; b += kPromptBatch) {
         p.batch = std::min(kPromptBatch, batch - b);
+        p.before = b;
         p.cu_q = cu_q + b; p.cu_k = cu_k + b;
         const int64_t most = ((int64_t)total_q / (2 * p.tokens) + p.batch) * kv_heads;
         if (most > (1 << 30)) return set_error(NCM_EUNSUPPORTED, "too many blocks of queries");

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_gpu_paged import DT, U, Cache, attend, attend64 as attend_one, int32
-from test_gpu_prompt import E, attend as attend_prompt, inputs, starts
+from test_gpu_prompt import E, attend as attend_prompt, attend64 as attend_all, check as check_prompt, inputs, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,49 @@ def test_prompt_all_scores_minus_infinity_over_values_that_are_not_finite(ncm, c
         assert bool((out[60:610] == 0).all())
         if causal:
             assert torch.equal(out[:60], good[:60]) and torch.equal(out[610:], good[610:])
+
+
+def cut(cu, total):
+    """Starts raised to the largest before them and cut to the range."""
+    out = []
+    for x in cu:
+        out.append(min(max([x, 0] + out), total))
+    return out
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 1, 128), (8, 2, 64)])
+@pytest.mark.parametrize("cu", [[0, 2000, 0, 2000], [0, 1000, 20, 1500, 1400], [0, 1700, 5, 1800, 6, 1900, 7, 1950], [300, 200, 900, 2 ** 31 - 1, 0, 2000],
+                                [-5, 700, -2 ** 31, 1200]])
+def test_prompt_falling_starts(ncm, cuda, heads, kvh, hd, cu):
+    """A sequence whose start falls below an earlier one's end begins there: rows have one sequence
+    each, the sound ones are right, and rows of none are left alone."""
+    total, err = 2000, int32([0])
+    q, k, v = inputs([total], [total], heads, kvh, hd, "bf16", seed=len(cu))
+    clean = cut(cu, total)
+    lk = [200 + 7 * i for i in range(len(cu) - 1)]
+    k, v = k[:sum(lk)], v[:sum(lk)]
+    lq, a = [y - x for x, y in zip(clean, clean[1:])], clean[0]
+    for causal in (False, True):
+        err.zero_()
+        out = attend_prompt(ncm, q, k, v, int32(cu), int32(starts(lk)), "bf16", causal, err=err)
+        assert err.item() == ncm.DEVICE_BAD_ARG
+        assert bool((out[:a] == 7).all()) and bool((out[clean[-1]:] == 7).all())
+        check_prompt(q[a:], k, v, out[a:], lq, lk, "bf16", causal)
+
+
+def test_prompt_falling_starts_of_many_sequences(ncm, cuda):
+    """The same where the sequences take several launches."""
+    batch, total, err = 2500, 5000, int32([0])
+    cu = [2 * i for i in range(batch + 1)]
+    cu[700], cu[1024], cu[1500], cu[1501] = 4000, 3, 100, 0
+    q, k, v = inputs([total], [total], 4, 2, 64, "f16", seed=3)
+    clean = cut(cu, total)
+    lk = [1 + i % 3 for i in range(batch)]
+    lk[-1] += total - sum(lk) if sum(lk) < total else 0
+    ck = starts(lk)
+    out = attend_prompt(ncm, q, k, v, int32(cu), int32(ck), "f16", False, err=err)
+    assert err.item() == ncm.DEVICE_BAD_ARG
+    for i in list(range(0, batch, 83)) + [698, 699, 700, 1023, 1024, 1025, 1499, 1500, 1501, 1999, 2000, 2001, 2047, 2048, 2049, 2499]:
+        a, b = clean[i], clean[i + 1]
+        ref, tol = attend_all(q[a:b], k[ck[i]:ck[i + 1]], v[ck[i]:ck[i + 1]], 0.125, None, "f16")
+        assert bool(((out[a:b].double() - ref).abs() <= tol).all()), i
