@@ -143,8 +143,10 @@ typedef struct {
 
 /* Writes `tokens` new rows into the cache and rotates q on the way.  Row i belongs to the
  * sequence s with cu_tokens[s] <= i < cu_tokens[s+1] (cu_tokens NULL: sequence i, one row
- * each); rows outside are padding and left alone.  lengths[s] counts the cached tokens
- * including the new ones, so that the last new row has position lengths[s] - 1.
+ * each); rows outside are padding and left alone.  Entries of cu_tokens lie
+ * from 0 to tokens and do not fall (NCM_DEVICE_BAD_ARG; a row is then stored where a sequence takes
+ * it by this definition, or nowhere).  lengths[s] counts the cached tokens including the new
+ * ones, so that the last new row has position lengths[s] - 1.
  *   q_out[i] = R(q[i]);  cache K[pos] = R(k[i]);  cache V[pos] = v[i]
  * in f32 (unfused multiplies and adds), rounded once.  q, k, v are of in_type (F32, F16 or
  * BF16), rows of heads x head_dim, consecutive rows *_stride elements apart (0: dense), so

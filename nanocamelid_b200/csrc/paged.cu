@@ -100,8 +100,9 @@ __device__ __forceinline__ int place_of_token(const int* cu, const int* lengths,
     const int first = __ldg(cu + at), end = __ldg(cu + at + 1), length = __ldg(lengths + at);
     const int k = __popc(__ballot_sync(NCM_FULL, lane < n && end <= token));
     if (k >= n) return -1;
-    pos = __shfl_sync(NCM_FULL, length - end + token, k);
-    return __shfl_sync(NCM_FULL, first, k) <= token ? lo + k : -1;   // before the first sequence
+    pos = __shfl_sync(NCM_FULL, max(length, 0) - (end - token), k);
+    // not so before the first sequence, nor for starts that are out of order
+    return __shfl_sync(NCM_FULL, (int)(first <= token && token < end), k) ? lo + k : -1;
 }
 
 template <typename T> __device__ __forceinline__ void load8(const T* p, float* x);
@@ -174,6 +175,10 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
     int off = 0, page = -1;
     float4 turn[4];                        // two (sin, cos) each, of the thread's eight pairs
     bool ready = false;
+    // The first CTA looks over the starts; the first of them are on their way with the rows.
+    const bool looks = p.cu && token == 0;
+    int cu0 = 0, cu1 = 0;
+    if (looks && threadIdx.x < p.batch) { cu0 = __ldg(p.cu + threadIdx.x); cu1 = __ldg(p.cu + threadIdx.x + 1); }
     for (int base = 0; base < all; base += blockDim.x) {
         const int task = base + threadIdx.x;
         const bool active = task < all;
@@ -189,6 +194,15 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
         }
         if (!ready) {
             ready = true;
+            if (looks) {
+                bool bad = cu0 < 0 || cu1 < cu0 || cu1 > p.tokens;
+                for (int b = threadIdx.x + blockDim.x; b < p.batch; b += blockDim.x) {
+                    cu0 = __ldg(p.cu + b); cu1 = __ldg(p.cu + b + 1);
+                    bad |= cu0 < 0 || cu1 < cu0 || cu1 > p.tokens;
+                }
+                if (bad) set_dev_error(p.err, NCM_DEVERR_BAD_ARG);
+                __syncwarp();
+            }
             int seq = token, pos = 0;
             if (p.cu) {
                 seq = place_of_token(p.cu, p.lengths, p.batch, token, pos);

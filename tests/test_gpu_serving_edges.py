@@ -183,3 +183,55 @@ def test_prompt_falling_starts_of_many_sequences(ncm, cuda):
         a, b = clean[i], clean[i + 1]
         ref, tol = attend_all(q[a:b], k[ck[i]:ck[i + 1]], v[ck[i]:ck[i + 1]], 0.125, None, "f16")
         assert bool(((out[a:b].double() - ref).abs() <= tol).all()), i
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 3, 2, 8], [0, 9, 1, 2, 8], [0, -3, 2, 2, 8], [0, 2, 4, 6, 9], [2 ** 31 - 1, -2 ** 31, 0, 0, 8],
+                                [0, 2, 4, 2 ** 31 - 1, 8], [-1, 2, 4, 6, 8]])
+def test_append_bad_starts_are_flagged(ncm, cuda, cu):
+    """Starts that fall or lie out of range: flagged, and a row is stored only where the sequence that
+    the definition gives it to (cu[s] <= i < cu[s + 1]) has its place."""
+    batch, tokens, heads, kvh, hd, page = 4, 8, 2, 1, 64, 8
+    totals = [20, 25, 30, 35]
+    c = Cache(ncm, "bf16", kvh, hd, page, [48] * batch, seed=3)
+    rows, err = torch.randn((tokens, heads + 2 * kvh, hd), generator=c.g, device="cuda").bfloat16(), int32([0])
+    keep, out = (int32(cu), int32(totals)), torch.full((tokens, heads, hd), 9.0, device="cuda").bfloat16()
+    w, es = (heads + 2 * kvh) * hd, 2
+    ncm.paged_append(c.kv, ncm.BF16, rows.data_ptr(), rows.data_ptr() + es * heads * hd, rows.data_ptr() + es * (heads + kvh) * hd, out.data_ptr(),
+                     ncm.BF16, tokens, heads, batch, keep[0].data_ptr(), keep[1].data_ptr(), c.table.data_ptr(), c.width, q_stride=w, k_stride=w,
+                     v_stride=w, err_ptr=err.data_ptr())
+    torch.cuda.synchronize()
+    assert err.item() == ncm.DEVICE_BAD_ARG
+    allowed = torch.zeros((c.pages, page), dtype=torch.bool, device="cuda")
+    for s in range(batch):
+        for i in range(tokens):
+            if cu[s] <= i < cu[s + 1]:
+                pos = totals[s] - cu[s + 1] + i
+                if 0 <= pos < 48:
+                    allowed[c.table[s, pos // page].item(), pos % page] = True
+    written = ~c.k[:, 0, :, 0].isnan()
+    assert not bool((written & ~allowed).any())
+
+
+@pytest.mark.parametrize("batch", [3, 33, 700, 1500])
+def test_append_falling_start_anywhere_is_flagged(ncm, cuda, batch):
+    tokens = 2 * batch
+    c = Cache(ncm, "f16", 1, 64, 8, [8] * batch, seed=batch)
+    rows, err = torch.randn((tokens, 3, 64), generator=c.g, device="cuda").half(), int32([0])
+    cu, lengths, out = int32([2 * i for i in range(batch + 1)]), int32([8] * batch), torch.zeros((tokens, 1, 64), device="cuda").half()
+
+    def call():
+        err.zero_()
+        ncm.paged_append(c.kv, ncm.F16, rows.data_ptr(), rows.data_ptr() + 128, rows.data_ptr() + 256, out.data_ptr(), ncm.F16, tokens, 1, batch,
+                         cu.data_ptr(), lengths.data_ptr(), c.table.data_ptr(), 1, q_stride=192, k_stride=192, v_stride=192, err_ptr=err.data_ptr())
+        return err.item()
+
+    assert call() == 0
+    for at in {1, batch // 2, batch - 1}:
+        keep = cu[at].item()
+        cu[at] = keep + 3
+        assert call() == ncm.DEVICE_BAD_ARG
+        cu[at] = keep
+    cu[batch] += 1
+    assert call() == ncm.DEVICE_BAD_ARG
+    cu[batch] -= 1
+    assert call() == 0
