@@ -117,8 +117,8 @@ ncm_status ncm_attention_noalloc(float* out, const float* q, const float* k_cach
  * a sequence's page table lists its pages in order (page_table[sequence][table_width]).
  * The calls below are stream ordered, allocate nothing and do not synchronise, so they can
  * be captured into a CUDA graph; lengths, page tables and cu_* arrays are read on the
- * device.  All pointers must be device memory of the current device (checked: NCM_EINVAL),
- * and `stream` one of its streams.  16-bit values are rounded to nearest.
+ * device.  All pointers must be device memory of the current device, int arrays 4-byte aligned
+ * (checked: NCM_EINVAL), and `stream` one of its streams.  16-bit values are rounded to nearest.
  *
  * What only the device can see is reported in *err (device int, zeroed by the caller; may
  * be NULL), whose bits are or-ed: NCM_DEVICE_BAD_ARG for a position, length, cu_* entry or

@@ -1090,6 +1090,7 @@ int log2_of(int v) {
     return n;
 }
 bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
+bool aligned4(const void* p) { return (((uintptr_t)p) & 3) == 0; }
 bool is_16bit(int t) { return t == NCM_TYPE_F16 || t == NCM_TYPE_BF16; }
 
 // What every call on a cache checks; null when it is sound.
@@ -1207,6 +1208,7 @@ extern "C" ncm_status ncm_paged_append(const ncm_paged_kv* kv, int in_type, cons
             return bad("q, k and v rows must be 16-byte aligned and at least a token apart");
     }
     if (!aligned16(q_out)) return bad("q_out must be 16-byte aligned");
+    if (!aligned4(cu_tokens) || !aligned4(lengths) || !aligned4(page_table) || !aligned4(err)) return bad("int arrays must be 4-byte aligned");
     const void* check[] = {k, v, kv->k, kv->v, kv->k_scales, kv->v_scales, lengths, page_table, cu_tokens, rope, src[0],
                            heads ? q_out : nullptr, err};
     if (const char* e = device_pointers_error(check, sizeof check / sizeof *check)) return bad(e);
@@ -1262,6 +1264,7 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     if (q_stride < wide || out_stride < wide || q_stride % 8 || out_stride % 8 || q_stride > ((int64_t)1 << 40) ||
         out_stride > ((int64_t)1 << 40) || !aligned16(q) || !aligned16(out) || !aligned16(workspace))
         return bad("q and out rows must be 16-byte aligned and at least a token apart");
+    if (!aligned4(lengths) || !aligned4(page_table) || !aligned4(err)) return bad("int arrays must be 4-byte aligned");
     size_t need = 0;
     if (ncm_paged_attention_workspace(heads, kv->kv_heads, hd, &need) || workspace_bytes < need)
         return bad("workspace smaller than ncm_paged_attention_workspace says");

@@ -737,6 +737,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
 
 // ------------------------------------------------------------------ host side
 bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
+bool aligned4(const void* p) { return (((uintptr_t)p) & 3) == 0; }
 int bad(const char* what) { return set_error(NCM_EINVAL, what); }
 
 bool kv_map(CUtensorMap* m, const void* base, int hd, int kv_heads, int tokens, int64_t stride) {
@@ -791,6 +792,7 @@ extern "C" ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const 
         if (*stride[i] < wide || *stride[i] % 8 || *stride[i] > ((int64_t)1 << 38) || !aligned16(at[i]))
             return bad("rows must be 16-byte aligned and at least a token apart");
     }
+    if (!aligned4(cu_q) || !aligned4(cu_k) || !aligned4(err)) return bad("int arrays must be 4-byte aligned");
     if (total_k == 0) { k = q; v = q; k_stride = q_stride; v_stride = q_stride; }   // never read: no row sees a key
     const void* check[] = {out, q, k, v, cu_q, cu_k, err};
     if (const char* e = device_pointers_error(check, sizeof check / sizeof *check)) return bad(e);

@@ -100,3 +100,14 @@ def test_host_memory(ncm):
     at = (ctypes.addressof(host) + 255) & ~255
     for text in (reason(ncm, attend, cache(ncm), out_ptr=at), reason(ncm, append, cache(ncm), q_ptr=at), reason(ncm, prompt, k_ptr=at)):
         assert text.split(": ", 1)[1] in POINTERS
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_int_arrays_off_their_alignment(ncm, off):
+    """They are read as ints: an odd address would be a misaligned access on the device."""
+    for name in ("cu_tokens_ptr", "lengths_ptr", "page_table_ptr", "err_ptr"):
+        assert "4-byte aligned" in reason(ncm, append, cache(ncm), **{name: P + off})
+    for name in ("lengths_ptr", "page_table_ptr", "err_ptr"):
+        assert "4-byte aligned" in reason(ncm, attend, cache(ncm), **{name: P + off})
+    for name in ("cu_q_ptr", "cu_k_ptr", "err_ptr"):
+        assert "4-byte aligned" in reason(ncm, prompt, **{name: P + off})
