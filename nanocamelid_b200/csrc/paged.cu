@@ -1253,7 +1253,7 @@ extern "C" ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int
     if (!is_16bit(q_type)) return bad("q_type must be F16 or BF16");
     if (kv->type != NCM_TYPE_Q8_0 && kv->type != q_type) return bad("q and a 16-bit cache must be of one type");
     if (batch < 0 || heads < 1 || heads > 65536 || heads % kv->kv_heads || table_width < 0) return bad("bad attention sizes");
-    if (!(scale >= 0.0f) || scale > 3.0e38f) return bad("scale must be positive (0: 1 / sqrt(head_dim))");
+    if (!(scale >= 0.0f) || scale > 2.0e38f) return bad("scale must be positive, below 2e38 (0: 1 / sqrt(head_dim))");
     if (batch == 0) return NCM_OK;
     if (!out || !q || !lengths || !page_table || !workspace) return bad("null pointer");
     if (table_width < 1 || (int64_t)table_width * kv->page_size > (1 << 22))

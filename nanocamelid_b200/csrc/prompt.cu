@@ -780,7 +780,7 @@ extern "C" ncm_status ncm_prompt_attention(void* out, int64_t out_stride, const 
     if (heads < 1 || kv_heads < 1 || kv_heads > 1024 || heads % kv_heads || heads / kv_heads > 128)
         return bad("heads must be a multiple of kv_heads, 128 to one at most");
     if (total_q < 0 || total_k < 0 || batch < 0 || total_q > (1 << 30) || total_k > (1 << 30)) return bad("bad prompt sizes");
-    if (!(scale >= 0.0f) || scale > 3.0e38f) return bad("scale must be positive (0: 1 / sqrt(head_dim))");
+    if (!(scale >= 0.0f) || scale > 2.0e38f) return bad("scale must be positive, below 2e38 (0: 1 / sqrt(head_dim))");
     if (total_q == 0 || batch == 0) return NCM_OK;
     if (!out || !q || !cu_q || !cu_k || (total_k && (!k || !v))) return bad("null pointer");
     const int64_t wide_q = (int64_t)heads * head_dim, wide_k = (int64_t)kv_heads * head_dim;

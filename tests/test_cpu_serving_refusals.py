@@ -111,3 +111,10 @@ def test_int_arrays_off_their_alignment(ncm, off):
         assert "4-byte aligned" in reason(ncm, attend, cache(ncm), **{name: P + off})
     for name in ("cu_q_ptr", "cu_k_ptr", "err_ptr"):
         assert "4-byte aligned" in reason(ncm, prompt, **{name: P + off})
+
+
+def test_scale_that_overflows_with_the_logarithm(ncm):
+    """The kernels take the scale times log2(e), which is infinite from 2.36e38 on."""
+    assert "scale must" in reason(ncm, attend, cache(ncm), scale=2.5e38)
+    assert "scale must" in reason(ncm, prompt, scale=2.5e38)
+    assert "scale" not in reason(ncm, attend, cache(ncm), scale=1.9e38) and "scale" not in reason(ncm, prompt, scale=1.9e38)
