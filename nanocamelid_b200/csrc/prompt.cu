@@ -615,8 +615,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attn_kernel(const __
                 const float now = max3(max3(m[0], m[1], m[2]), m[3], -INFINITY) * p.scale_log2;
                 // The maximum is moved only where a score has passed it by more than 2^8, so that
                 // the sums in TMEM are rarely rescaled; p stays below 2^8.  A score that is NaN or
-                // infinite makes the row NaN.
-                const bool over = !(now <= top + 8.0f);
+                // infinite makes the row NaN.  Rows of no token (behind the sequence, or where the group
+                // does not divide 128, whose queries are whatever lay there) have no say.
+                const bool over = mine && !(now <= top + 8.0f);
                 if (__any_sync(NCM_FULL, over)) {
                     const float a = !over ? 1.0f : now < INFINITY ? ex2(top - now) : NAN;
                     if (over && now < INFINITY) top = now;

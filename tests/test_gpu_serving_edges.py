@@ -235,3 +235,30 @@ def test_append_falling_start_anywhere_is_flagged(ncm, cuda, batch):
     assert call() == ncm.DEVICE_BAD_ARG
     cu[batch] -= 1
     assert call() == 0
+
+
+def test_prompt_rows_of_no_token_cost_nothing(ncm, cuda):
+    """A group of 12 fills 120 of a tile's 128 rows; the others hold what an earlier kernel left in
+    shared memory.  NaN there changes no output, and no time: the sums were rescaled at every step
+    for them, which took 1.7 times as long (1.02 without; the best of 20 each)."""
+    def call(heads, n, fill):
+        q, k, v = inputs([n], [n], heads, 8, 128, "bf16", seed=1)
+        if fill is not None:
+            q.fill_(fill)
+        cu, out = int32([0, n]), torch.empty_like(q)
+        return lambda: attend_prompt(ncm, q, k, v, cu, cu, "bf16", True, out=out, stream=torch.cuda.current_stream().cuda_stream)
+
+    f, before, best, outs = call(96, 4000, None), [call(32, 6000, x) for x in (0.0, float("nan"))], [1e9, 1e9], [None, None]
+    f()
+    for _ in range(20):
+        for i in range(2):
+            before[i]()
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = f()
+            b.record()
+            outs[i] = out.clone()
+            torch.cuda.synchronize()
+            best[i] = min(best[i], a.elapsed_time(b))
+    assert torch.equal(*outs)
+    assert best[1] < 1.3 * best[0], best
