@@ -7,7 +7,7 @@ value of at most 127, for each of the 32."""
 import pytest
 import torch
 
-from test_gpu_paged import DT, U, Cache, attend, attend64 as attend_one, int32
+from test_gpu_paged import DT, U, Cache, append, attend, attend64 as attend_one, check as check_one, check_append, int32, rope_table
 from test_gpu_prompt import E, attend as attend_prompt, attend64 as attend_all, check as check_prompt, inputs, starts
 
 pytestmark = pytest.mark.gpu
@@ -262,3 +262,134 @@ def test_prompt_rows_of_no_token_cost_nothing(ncm, cuda):
             best[i] = min(best[i], a.elapsed_time(b))
     assert torch.equal(*outs)
     assert best[1] < 1.3 * best[0], best
+
+
+def test_host_pointers_are_told_from_sound_ones(ncm, cuda):
+    """Calls that succeed, and then each of their pointers in turn in host memory, refused for that."""
+    host = torch.zeros(1 << 16, dtype=torch.uint8).pin_memory().data_ptr()
+    space = torch.zeros(ncm.paged_attention_workspace(2, 1, 64), dtype=torch.uint8, device="cuda")
+    x = [torch.ones(16 * 64 * 4, dtype=torch.float16, device="cuda") for _ in range(8)]
+    q, k, v, out, pk, pv, sk, sv = (t.data_ptr() for t in x)
+    starts_, lengths, table, err = int32([0, 1]), int32([1]), int32([0]), int32([0])
+    rope = torch.ones((1, 32, 2), device="cuda")
+
+    def each(f, base, names):
+        f(**base)
+        torch.cuda.synchronize()
+        assert err.item() == 0
+        for name in names or [n for n in base if n.endswith("_ptr")]:
+            with pytest.raises(ncm.NcmError, match="not a device pointer"):
+                f(**{**base, name: host})
+
+    kv = ncm.PagedKV(ncm.F16, pk, pv, 4, 16, 1, 64)
+    each(lambda **a: ncm.paged_append(kv, **a),
+         dict(in_type=ncm.F16, q_ptr=q, k_ptr=k, v_ptr=v, q_out_ptr=out, q_out_type=ncm.F16, tokens=1, heads=2, batch=1, cu_tokens_ptr=starts_.data_ptr(),
+              lengths_ptr=lengths.data_ptr(), page_table_ptr=table.data_ptr(), table_width=1, rope_ptr=rope.data_ptr(), rope_len=1, rope_half=32,
+              err_ptr=err.data_ptr()), None)
+    decode = dict(q_type=ncm.F16, batch=1, heads=2, lengths_ptr=lengths.data_ptr(), page_table_ptr=table.data_ptr(), table_width=1,
+                  workspace_ptr=space.data_ptr(), workspace_bytes=space.numel(), err_ptr=err.data_ptr())
+    each(lambda out_ptr=out, q_ptr=q, **a: ncm.paged_attention(out_ptr, q_ptr, kv, **a), {**decode, "out_ptr": out, "q_ptr": q}, None)
+
+    def over(k=pk, v=pv, k_scales=sk, v_scales=sv, **a):
+        ncm.paged_attention(out, q, ncm.PagedKV(ncm.Q8_0, k, v, 4, 16, 1, 64, k_scales, v_scales), **a)
+
+    each(over, decode, ["k", "v", "k_scales", "v_scales"])
+    each(lambda **a: ncm.prompt_attention(**a),
+         dict(out_ptr=out, q_ptr=q, k_ptr=k, v_ptr=v, type=ncm.F16, total_q=1, total_k=1, batch=1, heads=2, kv_heads=1, head_dim=64,
+              cu_q_ptr=starts_.data_ptr(), cu_k_ptr=starts_.data_ptr(), err_ptr=err.data_ptr()), None)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(65, 1, 64), (100, 1, 128), (127, 1, 128), (128, 1, 64), (256, 2, 128), (43, 1, 64)])
+def test_prompt_wide_groups(ncm, cuda, kind, heads, kvh, hd):
+    """One to a few tokens to a tile."""
+    lq, lk = [5, 0, 1, 40], [5, 3, 200, 333]
+    q, k, v = inputs(lq, lk, heads, kvh, hd, kind, seed=heads, rows_behind=2)
+    for causal in (True, False):
+        out = attend_prompt(ncm, q, k, v, int32(starts(lq)), int32(starts(lk)), kind, causal)
+        check_prompt(q, k, v, out, lq, lk, kind, causal)
+        assert bool((out[sum(lq):] == 7).all())
+
+
+@pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("q8_0", "f16")])
+@pytest.mark.parametrize("heads,kvh,hd", [(17, 1, 64), (33, 1, 128), (128, 1, 128), (100, 2, 64), (600, 600, 64)])
+def test_attention_wide_groups(ncm, cuda, kind, qkind, heads, kvh, hd):
+    """Groups that make several segments, and many key-value heads."""
+    lengths = [0, 1, 33, 700] if kvh < 600 else [3, 40]
+    c = Cache(ncm, kind, kvh, hd, 16, lengths, seed=heads).fill()
+    q = torch.randn((len(lengths), heads, hd), generator=c.g, device="cuda").to(DT[qkind])
+    check_one(c, q, attend(ncm, c, q, int32(lengths), heads, qkind), lengths, qkind)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_q8_outlier_channel_in_q(ncm, cuda, hd):
+    """One value of a block of q many times the others, which its integers are multiples of."""
+    lengths, heads, kvh = [40, 2000], 8, 2
+    c = Cache(ncm, "q8_0", kvh, hd, 32, lengths, seed=4).fill()
+    for times in (20, 1000):
+        q = torch.randn((2, heads, hd), generator=c.g, device="cuda")
+        q[:, :, 37] *= times
+        q = q.half()
+        check_one(c, q, attend(ncm, c, q, int32(lengths), heads, "f16"), lengths, "f16")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_q8_pages_of_keys_and_values_side_by_side(ncm, cuda, hd):
+    """A Q8_0 cache in one allocation with a page stride: append, then attention."""
+    heads, kvh, page, totals = 8, 2, 16, [50, 3, 130]
+    c = Cache(ncm, "q8_0", kvh, hd, page, totals, seed=2)
+    both = torch.full((c.pages, 2, kvh, page, hd), 127, dtype=torch.int8, device="cuda")
+    c.k, c.v = both[:, 0], both[:, 1]
+    c.kv = ncm.PagedKV(ncm.Q8_0, c.k.data_ptr(), c.v.data_ptr(), c.pages, page, kvh, hd, c.ks.data_ptr(), c.vs.data_ptr(), 2 * kvh * page * hd)
+    before = [x.clone() for x in (c.k, c.v, c.ks, c.vs)]
+    rows = torch.randn((sum(totals), heads + 2 * kvh, hd), generator=c.g, device="cuda").half()
+    rope = rope_table(200, hd // 2, hd)
+    out = append(ncm, c, rows, heads, totals, totals, "f16", "f16", rope, "halves", hd // 2)
+    check_append(c, rows, heads, totals, totals, "f16", rope, "halves", hd // 2, out, before)
+    q = out[[49, 52, 182]].contiguous()
+    check_one(c, q, attend(ncm, c, q, int32(totals), heads, "f16"), totals, "f16")
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("inkind", ["f32", "bf16"])
+def test_append_many_tokens_in_several_passes(ncm, cuda, kind, inkind):
+    """So many tokens that a CTA takes each in passes of 128 threads."""
+    counts, totals, heads, kvh, hd = [700, 1, 0, 333], [700, 50, 9, 400], 24, 6, 128
+    c = Cache(ncm, kind, kvh, hd, 32, totals, seed=6)
+    before = [x.clone() if x is not None else None for x in (c.k, c.v, c.ks, c.vs)]
+    rows = (torch.randn((sum(counts) + 5, heads + 2 * kvh, hd), generator=c.g, device="cuda") * 2).to(DT[inkind])
+    rope = rope_table(700, 64, hd)
+    out = append(ncm, c, rows, heads, counts, totals, "bf16", inkind, rope, "pairs", 64)
+    check_append(c, rows, heads, counts, totals, "bf16", rope, "pairs", 64, out, before)
+
+
+def test_rows_and_pages_past_32_bits(ncm, cuda):
+    """Elements past 2^31 and bytes past 2^32 of each operator's rows, and of the append's pages."""
+    heads, kvh, hd, n, apart = 4, 2, 64, 100, 1 << 25
+    wide = torch.zeros(n * apart, dtype=torch.float16, device="cuda").view(n, apart)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide[:, :2 * heads * hd + 2 * kvh * hd] = torch.randn((n, 2 * heads * hd + 2 * kvh * hd), generator=g, device="cuda").half()
+    at = [0, heads * hd, (heads + kvh) * hd, (heads + 2 * kvh) * hd]
+    q, k, v, out = (wide[:, a:a + h * hd].unflatten(1, (h, hd)) for a, h in zip(at, (heads, kvh, kvh, heads)))
+    cu = int32([0, 30, n])
+    ncm.prompt_attention(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), ncm.F16, n, n, 2, heads, kvh, hd, cu.data_ptr(), cu.data_ptr(),
+                         q_stride=apart, k_stride=apart, v_stride=apart, out_stride=apart)
+    check_prompt(q, k, v, out, [30, 70], [30, 70], "f16", True)
+    page = 8
+    pages = 2 ** 31 // (kvh * page * hd) + 20
+    c = Cache(ncm, "f16", kvh, hd, page, [60, 60], seed=1)
+    c.k, c.v = (torch.full((pages, kvh, page, hd), 3.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    c.pages, c.kv = pages, ncm.PagedKV(ncm.F16, c.k.data_ptr(), c.v.data_ptr(), pages, page, kvh, hd)
+    c.table = torch.randperm(16, generator=g, device="cuda").to(torch.int32).view(2, 8).contiguous()
+    c.table[:, 4:] += pages - 16
+    cu, lengths, q_out, err = int32([0, 40, n]), int32([40, 60]), torch.zeros((n, heads, hd), dtype=torch.float16, device="cuda"), int32([0])
+    ncm.paged_append(c.kv, ncm.F16, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), ncm.F16, n, heads, 2, cu.data_ptr(), lengths.data_ptr(),
+                     c.table.data_ptr(), 8, q_stride=apart, k_stride=apart, v_stride=apart, err_ptr=err.data_ptr())
+    assert err.item() == 0 and torch.equal(q_out, q)
+    assert torch.equal(c.rows("k", 0, 40), k[:40].double()) and torch.equal(c.rows("v", 1, 60), v[40:].double())
+    space = torch.zeros(ncm.paged_attention_workspace(heads, kvh, hd), dtype=torch.uint8, device="cuda")
+    ncm.paged_attention(out[39].data_ptr(), q[39].data_ptr(), c.kv, ncm.F16, 2, heads, lengths.data_ptr(), c.table.data_ptr(), 8, space.data_ptr(),
+                        space.numel(), q_stride=60 * apart, out_stride=60 * apart)
+    for i, row in enumerate((39, 99)):
+        ref, tol = attend_one(q[row], c.rows("k", i, (40, 60)[i]), c.rows("v", i, (40, 60)[i]), hd ** -0.5, "f16", hd)
+        assert bool(((out[row].double() - ref).abs() <= tol).all())
