@@ -157,7 +157,8 @@ typedef struct {
  * NCM_ROPE_PAIRS rotates (2i, 2i+1) for i < rope_half (inference.rs:904-933), the rest passes
  * unchanged; NCM_ROPE_HALVES rotates (i, i + head_dim/2), rope_half = head_dim/2.
  * Q8_0: per 32 values scale = max|x| * (1 / 127) in f32, kept as f16 rounded toward zero, int8 =
- * round-half-away(x * (1 / scale)): ncm_model_set_kv_cache's rule but for its division.
+ * round-half-away(x * (1 / scale)): ncm_model_set_kv_cache's rule but for its division
+ * by 127 (of 2 million random blocks fewer than 10 differ, each in int8 values by one).
  * A row whose position or page is out of range is not written at all (NCM_DEVICE_BAD_ARG). */
 #define NCM_ROPE_PAIRS 0
 #define NCM_ROPE_HALVES 1
@@ -205,7 +206,8 @@ ncm_status ncm_paged_attention(const ncm_paged_kv* kv, void* out, int64_t out_st
  * q and out: [total_q][heads][head_dim], k and v: [total_k][kv_heads][head_dim], of `type` (F16
  * or BF16), tokens *_stride elements apart (0: dense), 16-byte aligned; head_dim 64 or 128, at
  * most 128 query heads to a key-value head; out may not overlap an input.  scale 0 means
- * 1 / sqrt(head_dim).  An entry of cu_q below an earlier one counts as that one, an entry of
+ * 1 / sqrt(head_dim).  A sequence may have 2^26 keys (more can run into the limit of a wait:
+ * NCM_DEVICE_TIMEOUT).  An entry of cu_q below an earlier one counts as that one, an entry of
  * cu_* below 0 or past total_q / total_k as that border, and where cu_k falls a sequence has no keys
  * (NCM_DEVICE_BAD_ARG).  Runs on tcgen05; p is rounded to `type` as by
  * ncm_paged_attention, sums are f32. */

@@ -376,8 +376,7 @@ struct Place {
     int b, hk, u, n;   // sequence, segment within it, unit within the segment, units of the segment
 };
 
-// out (f32) = the weighted sum of `n` parts: each has a maximum and a sum per head and a row of
-// hd sums.  A part whose sum is zero counts for nothing whatever its maximum is.
+// Four values of out, from `at` on, rounded to its 16-bit type.
 template <bool BF16>
 __device__ __forceinline__ void store_out(void* out, int64_t at, float4 v) {
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(pack2(BF16, v.x, v.y), pack2(BF16, v.z, v.w));
@@ -389,6 +388,8 @@ __device__ __forceinline__ float scaled(float v, float inv) { return inv == 0.0f
 __device__ __forceinline__ float4 scaled(float4 v, float inv) {
     return make_float4(scaled(v.x, inv), scaled(v.y, inv), scaled(v.z, inv), scaled(v.w, inv));
 }
+// What a part (a maximum and a sum per head, and a row of hd sums) counts in a join whose largest
+// maximum is `top`: nothing if none of its keys scored above -infinity.
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 0.0f : ex2(m - top); }
 
 __host__ __device__ constexpr bool one_stage(bool q8, int hd, int nt) { return nt == 1 && (hd == 128 || !q8); }
@@ -1163,11 +1164,18 @@ int paged_attn_run(PagedAttnParams& p, int grid, cudaStream_t s) {
 template <bool BF16, bool Q8>
 int paged_attn_pick(PagedAttnParams& p, int hd, int grid, cudaStream_t s) {
     const bool two = p.chunk > 8;
-    // Warps of a CTA.  Q8_0 is bound by instructions and takes as many as its registers allow (48
-    // sequences of 300 to 6000, 32 / 8 heads of 128: 8 warps 79.9 us, 12 77.5; heads of 64: 8 86.1,
-    // 12 75.9, with one stage each 72.1 where the later 66.4 take three).  16-bit values need only
-    // enough in flight (64 sequences of 1 to 8192, heads of 128: 6 warps of two stages 177 us, 7 of one
-    // 168, 8 171, 9 175; 64 of 300 to 8000, heads of 64: 8 of three 87.4, 8 of one 83.0, 10 80.9, 12 81.7).
+    // Warps of a CTA.  Over Q8_0 each warp waits on its own instructions (0.53 issued a cycle and
+    // scheduler, no pipe above 28 %): as many as the registers allow without more stages falling out.
+    // 16-bit values need only enough in flight.  Measured in us, 32 / 8 heads but where said:
+    //   16-bit, heads of 128: 64 sequences of 1 to 8192  6 warps of two stages 166.6, 7 of one 168.9, 9 169.9;
+    //     48 of 300 to 6000  97.3, 95.0, 98.6; 4 of those  19.8, 18.4, 18.9
+    //   16-bit, heads of 64: 64 of 300 to 6000  8 warps 75.0, 10 75.1, 12 75.1; 64 of 300 to 8000  83.0,
+    //     80.9, 81.7; 4 of 300 to 6000  13.2, 14.0, 14.6
+    //   Q8_0, heads of 128: 48 of 300 to 6000  8 warps 77.5, 10 79.8, 12 71.1; 8 / 1 heads, 64 of them
+    //     26.2, 26.3, 26.0
+    //   Q8_0, heads of 64: 48 of 300 to 6000  10 warps 55.0, 12 50.4, 14 52.7
+    //   9 to 16 heads a segment, 48 of 300 to 6000: heads of 64 (12) 6 warps 64.6, 8 65.7, 10 65.3; Q8_0 (16) 94.9,
+    //     75.6, 81.2; heads of 128 (12) 3 warps 115, 4 110.7, 5 106.2; Q8_0 (16) 6 warps 137, 7 123, 8 109
     if (hd == 64)
         return two ? paged_attn_run<BF16, Q8, 64, 2, 8>(p, grid, s) : paged_attn_run<BF16, Q8, 64, 1, Q8 ? 12 : 10>(p, grid, s);
     if (two) return paged_attn_run<BF16, Q8, 128, 2, Q8 ? 8 : 4>(p, grid, s);

@@ -40,8 +40,10 @@ constexpr int kRows = 128;               // query rows of a tile, and keys of a 
 constexpr int kUnitKeys = 64;            // keys of one step of the softmax
 constexpr int kPromptThreads = 384;
 constexpr int kPromptBatch = 1024;       // sequences of one launch
-// Exponentials of every eight that the FMA pipe computes: 0, 1, 2, 3 take 107.5, 104.5, 102.1,
-// 103.5 us (12 ragged prompts, 32 / 8 heads of 64) and 146, 144, 143.5, 146 (4 chunks, 64 / 8 of 128).
+// Exponentials of every eight that the FMA pipe computes: 0, 1, 2, 3 take 106.7, 103.7, 101.5, 102.7
+// us for 12 ragged prompts, 32 / 8 heads of 64, in F16 and 108, 105 to 109, 101 to 105, 105 to 110 in BF16.
+// With heads of 128 (4 chunks over 4000 keys, 64 / 8) the power cap moves each from 145 to 156 in BF16
+// and from 162 to 182 in F16, and the four do not differ beyond that.
 constexpr int kPolyOf8 = 2;
 constexpr int kPromptSmem = 232448;
 constexpr uint64_t kPromptWaitNs = 2000000000ull;
@@ -225,7 +227,7 @@ struct Item {
 __device__ __forceinline__ Item item_at(const PromptParams& p, const int* prefix, int index) {
     const int *cu_q = prefix + p.batch + 1, *cu_k = cu_q + p.batch + 1;
     Item t;
-    const int block = prefix[p.batch] - 1 - index / p.kv_heads;   // the blocks that see most keys come first
+    const int block = prefix[p.batch] - 1 - index / p.kv_heads;   // of a causal sequence the blocks that see most keys come first
     t.head = index % p.kv_heads;
     int lo = 0, hi = p.batch;
     while (hi - lo > 1) {
