@@ -638,9 +638,12 @@ __global__ void __launch_bounds__(W * 32, 1) paged_attn_kernel(const __grid_cons
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[t][j] += __shfl_xor_sync(NCM_FULL, l[t][j], x);
+                // a score that overflowed makes the row NaN: beside it every p is zero
+                if (m[t][j] == INFINITY) l[t][j] = NAN;
+            }
     };
     auto keep = [&](float* rows, float* ml) {   // a part, in shared memory
 #pragma unroll

@@ -393,3 +393,23 @@ def test_rows_and_pages_past_32_bits(ncm, cuda):
     for i, row in enumerate((39, 99)):
         ref, tol = attend_one(q[row], c.rows("k", i, (40, 60)[i]), c.rows("v", i, (40, 60)[i]), hd ** -0.5, "f16", hd)
         assert bool(((out[row].double() - ref).abs() <= tol).all())
+
+
+def test_scores_that_overflow_are_not_zeros(ncm, cuda):
+    """A score past f32's range, by the scale or by itself, makes its row NaN in both operators."""
+    heads, kvh, hd = 4, 2, 64
+    for n in (7, 3000):
+        c = Cache(ncm, "bf16", kvh, hd, 16, [n, 40], seed=2).fill()
+        q = torch.randn((2, heads, hd), generator=c.g, device="cuda").bfloat16()
+        good = attend(ncm, c, q, int32([n, 40]), heads, "bf16", scale=30.0)
+        at = n // 2
+        page, off = c.table[0, at // 16].item(), at % 16
+        c.k[page, 1, off] = 2e18
+        q[0, 2:] = 1e18   # q.k = 1.3e38, times 30 past the range
+        for scale in (30.0, 1e10):
+            out = attend(ncm, c, q, int32([n, 40]), heads, "bf16", scale=scale)
+            assert bool(out[0, 2:].isnan().all())
+            assert scale != 30.0 or torch.equal(out[0, :2], good[0, :2]) and torch.equal(out[1], good[1])
+        k, v = c.rows("k", 0, n).bfloat16(), c.rows("v", 0, n).bfloat16()
+        out = attend_prompt(ncm, q[:1], k, v, int32([0, 1]), int32([0, n]), "bf16", True, scale=30.0)
+        assert bool(out[0, 2:].isnan().all())
